@@ -103,4 +103,10 @@ __device__ __forceinline__ f32x4 leaky4(f32x4 v, float slope) {
     return f32x4{vmax_raw(v[0], m[0]), vmax_raw(v[1], m[1]), vmax_raw(v[2], m[2]), vmax_raw(v[3], m[3])};
 }
 
+// Clears `words` 32-bit words with one small launch.  A kernel and not hipMemsetAsync: memset nodes of a captured HIP graph
+// have given wrong results on replays after the first.
+static __global__ void __launch_bounds__(64) clear_words_kernel(unsigned* p, int words) {
+    for (int i = threadIdx.x; i < words; i += 64) p[i] = 0u;
+}
+
 }  // namespace yolo

@@ -436,7 +436,7 @@ extern "C" int yolo_train_loss_fwd(const yolo_view* head, int L, const int* stri
     p.w_noobj = noobj_weight;
     p.losses = losses;
     hipStream_t st = (hipStream_t)stream;
-    YOLO_CHECK_HIP(hipMemsetAsync(p.counts, 0, 16, st));
+    hipLaunchKernelGGL(clear_words_kernel, dim3(1), dim3(64), 0, st, (unsigned*)p.counts, 4);
     hipLaunchKernelGGL(loss_gt_pick_kernel, dim3(N * K), dim3(256), 0, st, p);
     hipLaunchKernelGGL(loss_label_kernel, dim3(p.partial_blocks), dim3(256), 0, st, p);
     hipLaunchKernelGGL(loss_value_kernel, dim3(p.partial_blocks), dim3(256), 0, st, p);

@@ -1170,7 +1170,7 @@ extern "C" int yolo_batched_nms(const float* boxes, const float* scores, const i
     constexpr int SORT_LDS = (int)sizeof(SortShared);
     const void* const sort_kern[] = {(const void*)nms_sort_kernel};
     YOLO_CHECK_HIP(lds_limit.raise(sort_kern, 1, SORT_LDS));
-    YOLO_CHECK_HIP(hipMemsetAsync(p.nseg, 0, 256, st));
+    hipLaunchKernelGGL(clear_words_kernel, dim3(1), dim3(64), 0, st, p.nseg, 64);
     hipLaunchKernelGGL(nms_sort_kernel, dim3(N), dim3(SORT_THREADS), SORT_LDS, st, p);
     // one wave per segment; at most N * num_classes segments, and no more than candidates
     long long segs = (long long)N * num_classes;
