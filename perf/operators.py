@@ -181,7 +181,7 @@ def _own_clip(s, case):
 def _own_step(s, case):
     from yolo_amd import ops
     norm = s["clipper"].measure()
-    ops.sgd_step_clipped(s["param"], s["grad"], s["mom"], *s["blocks"], s["lr"], s["decay"], s["lr"], 0.0, s["momentum"],
+    ops.sgd_step_clipped(s["param"], s["grad"], s["mom"], s["blocks"], s["lr"], s["decay"], s["lr"], 0.0, s["momentum"],
                          coefs=s["clipper"].coefs)
     return {"norm": norm, "param": s["param"], "momentum": s["mom"]}
 
