@@ -34,6 +34,10 @@ extern "C" {
 #define YOLO_F32 0
 #define YOLO_BF16 1
 
+/* activations of yolo_gn_act_fwd / _bwd */
+#define YOLO_ACT_LEAKY 0 /* t > 0 ? t : slope * t (slope 1: none, slope 0: ReLU) */
+#define YOLO_ACT_SILU 1  /* t * sigmoid(t) */
+
 /* NMS modes, see yolo_batched_nms */
 #define YOLO_NMS_PER_CLASS 0   /* torchvision _batched_nms_vanilla */
 #define YOLO_NMS_COORD_TRICK 1 /* torchvision _batched_nms_coordinate_trick */
@@ -372,6 +376,59 @@ int yolo_pack_conv_train_batch(const yolo_pack_desc* descs_device, int n_layers,
  */
 int yolo_sgd_step(float* param, const float* grad, float* momentum_buf, const int* block_table, int n_blocks, float lr0,
                   float weight_decay0, float lr1, float weight_decay1, float momentum, void* stream);
+
+/*
+ * Group normalisation + activation [+ residual]: what detectron2's get_norm("GN") (torch.nn.GroupNorm) and the
+ * F.leaky_relu behind it compute for a convolution's output (the norm's name is MODEL.DARKNET.NORM, darknet.py:45-53,
+ * 74-106, fpn.py:23-30,44-61,78-90):
+ *   t = (x - mean) / sqrt(var + eps) * gamma[c] + beta[c],   y = act(t) [+ residual]
+ * with mean and (biased) var over the H*W*C/groups values of each image's group.
+ *   stats  [2][N][groups] f32: mean and 1 / sqrt(var + eps), which yolo_gn_act_bwd reads
+ * y may be x, and may be residual; C is a multiple of 8 and of groups; slope in [0, 1]; one image of a view is below 2 GiB.
+ * workspace: yolo_gn_workspace_bytes, enough for either direction, nothing is kept in it between calls.
+ */
+size_t yolo_gn_workspace_bytes(int N, int H, int W, int C, int groups, int dtype);
+int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const float* beta, const yolo_view* residual,
+                    const yolo_view* y, float* stats, int N, int C, int groups, float eps, int act, float leaky_slope,
+                    int dtype, void* workspace, size_t ws_bytes, void* stream);
+
+/* Backward of yolo_gn_act_fwd (without the residual, whose gradient is dy itself): from dy, the saved x and stats writes
+ * dx, and dgamma, dbeta [C] f32 (overwritten).  The leaky derivative at t == 0 is slope.  dx may be dy, and may be x. */
+int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const float* gamma, const float* beta, const float* stats,
+                    const yolo_view* dx, float* dgamma, float* dbeta, int N, int C, int groups, int act,
+                    float leaky_slope, int dtype, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Gradient norms and clipping over any number of tensors (detectron2's SOLVER.CLIP_GRADIENTS; torch.nn.utils
+ * .clip_grad_norm_ and clip_grad_value_).  A device table of runs says which elements a workgroup owns; the runs of one
+ * tensor follow each other.
+ */
+typedef struct yolo_grad_block {
+    void* ptr;    /* first element of the run */
+    int count;    /* elements, >= 1 */
+    int tensor;   /* which tensor the run belongs to */
+    int dtype;    /* YOLO_F32 or YOLO_BF16 */
+    int reserved;
+} yolo_grad_block;
+
+size_t yolo_grad_norm_workspace_bytes(int n_blocks);
+
+/* norms[0] = the norm over all runs; with tensor_first (device, [n_tensors + 1]: the tensors' first runs, then n_blocks)
+ * norms[t] = the norm of tensor t (0 for one without elements).  norm_type 1, 2 or INFINITY.  coefs (may be null), laid
+ * out like norms: min(1, max_norm / (norm + 1e-6)).  Sums are fp64, joined in the table's order. */
+int yolo_grad_norm(const yolo_grad_block* blocks, int n_blocks, const int* tensor_first, int n_tensors, float norm_type,
+                   float max_norm, float* norms, float* coefs, void* workspace, size_t ws_bytes, void* stream);
+/* g *= coefs[0], or coefs[tensor of the run] */
+int yolo_grad_scale(const yolo_grad_block* blocks, int n_blocks, const float* coefs, int per_tensor, void* stream);
+/* g = min(max(g, -value), value), a NaN stays */
+int yolo_grad_clamp(const yolo_grad_block* blocks, int n_blocks, float value, void* stream);
+
+/* yolo_sgd_step on clipped gradients: d = coefs[0 or the run's tensor] * grad, or with coefs null d = grad clamped to
+ * [-clip_value, clip_value]; grad itself is left as it is.  block_table (device): [n_blocks][4] i32 = first element, count,
+ * group (0 / 1), tensor.  The three arenas begin at 16-byte boundaries. */
+int yolo_sgd_step_clipped(float* param, const float* grad, float* momentum_buf, const int* block_table, int n_blocks,
+                          float lr0, float weight_decay0, float lr1, float weight_decay1, float momentum,
+                          const float* coefs, int per_tensor, float clip_value, void* stream);
 
 /*
  * Data gradient of a 3x3 / stride-2 / pad-1 convolution (ResidualBlock.downsample, darknet.py:79-82,113-116, under

@@ -1,0 +1,116 @@
+"""What the GroupNorm and gradient-clipping entry points refuse before any launch, and their host-side parts (no GPU)."""
+import ctypes
+
+import pytest
+import torch
+
+from yolo_amd import _lib, ops, solver
+
+
+def _view(H=8, W=8, halo=0, total=64, at=0, ptr=4096):
+    return _lib.YoloView(ptr, H, W, halo, total, at)
+
+
+def _fwd(x=None, y=None, r=None, N=1, C=64, groups=32, eps=1e-5, act=0, slope=0.1, dtype=1, ws=1 << 30, ptr=4096):
+    L = _lib.lib()
+    x, y = x or _view(), y or _view()
+    code = L.yolo_gn_act_fwd(ctypes.byref(x), ptr, ptr, ctypes.byref(r) if r else None, ctypes.byref(y), ptr, N, C, groups, eps,
+                             act, slope, dtype, ptr, ws, None)
+    return code, L.yolo_last_error().decode()
+
+
+def _bwd(dy=None, x=None, dx=None, N=1, C=64, groups=32, act=0, slope=0.1, dtype=1, ws=1 << 30, ptr=4096):
+    L = _lib.lib()
+    dy, x, dx = dy or _view(), x or _view(), dx or _view()
+    code = L.yolo_gn_act_bwd(ctypes.byref(dy), ctypes.byref(x), ptr, ptr, ptr, ctypes.byref(dx), ptr, ptr, N, C, groups, act,
+                             slope, dtype, ptr, ws, None)
+    return code, L.yolo_last_error().decode()
+
+
+@pytest.mark.parametrize("call", [_fwd, _bwd], ids=["fwd", "bwd"])
+@pytest.mark.parametrize("kw,says", [
+    (dict(ptr=None), "null"), (dict(x=_view(ptr=None)), "null"), (dict(x=_view(H=0)), "expected"), (dict(N=0), "batch"),
+    (dict(N=65536), "batch"), (dict(C=60), "channels"), (dict(C=0), "channels"), (dict(groups=0), "groups"),
+    (dict(groups=7), "groups"), (dict(act=2), "activation"), (dict(slope=-0.1), "slope"), (dict(slope=float("nan")), "slope"),
+    (dict(dtype=2), "dtype"), (dict(ws=16), "workspace"), (dict(x=_view(at=8)), "slice"), (dict(x=_view(total=68)), "slice"),
+    (dict(x=_view(ptr=4100)), "aligned"), (dict(x=_view(H=4096, W=4096, total=64)), "2 GiB")],
+    ids=lambda v: "-".join(v) if isinstance(v, dict) else v.replace(" ", ""))
+def test_gn_refusals(call, kw, says):
+    code, message = call(**kw)
+    assert code < 0 and says in message, message
+
+
+def test_gn_refusals_of_one_direction():
+    assert "y is 8 x 9" in _fwd(y=_view(W=9))[1] and "residual is 7 x 8" in _fwd(r=_view(H=7))[1]
+    assert "eps" in _fwd(eps=-1.0)[1] and "dy is 9 x 8" in _bwd(dy=_view(H=9))[1] and "dx is 8 x 4" in _bwd(dx=_view(W=4))[1]
+    assert _fwd(ws=16)[0] == -2
+    L = _lib.lib()
+    assert L.yolo_gn_workspace_bytes(0, 8, 8, 64, 32, 1) == 0 and L.yolo_gn_workspace_bytes(1, 8, 8, 60, 4, 1) == 0
+    assert L.yolo_gn_workspace_bytes(64, 208, 208, 64, 32, 1) > 0
+
+
+def test_grad_refusals():
+    L = _lib.lib()
+    p = 4096
+    inf = float("inf")
+    for args, says in (((p, 1, None, 0, 2.0, 1.0, None, p, p, 8), "null"), ((None, 1, None, 0, 2.0, 1.0, p, p, p, 8), "null"),
+                       ((p, -1, None, 0, 2.0, 1.0, p, p, p, 8), "blocks"), ((p, 1, p, 0, 2.0, 1.0, p, p, p, 8), "tensors"),
+                       ((p, 1, None, 0, 3.0, 1.0, p, p, p, 8), "norm type"), ((p, 1, None, 0, -inf, 1.0, p, p, p, 8), "norm type"),
+                       ((p, 1, None, 0, 2.0, -1.0, p, p, p, 8), "max_norm"), ((p, 2, None, 0, inf, 1.0, p, p, p, 8), "workspace")):
+        assert L.yolo_grad_norm(*args, None) < 0 and says in L.yolo_last_error().decode(), says
+    assert L.yolo_grad_scale(p, 1, None, 0, None) < 0 and L.yolo_grad_clamp(p, 1, -1.0, None) < 0
+    assert L.yolo_grad_clamp(p, 1, float("nan"), None) < 0
+    step = lambda w, n, coefs, v: L.yolo_sgd_step_clipped(w, p, p, p, n, 0.1, 0.0, 0.1, 0.0, 0.9, coefs, 0, v, None)  # noqa: E731
+    assert step(None, 1, p, 0.0) < 0 and step(p, 0, p, 0.0) < 0 and step(p, 1, None, -1.0) < 0 and step(p + 4, 1, p, 0.0) < 0
+
+
+def test_dense_runs():
+    t = torch.zeros(4, 6, 3, 3)
+    for v in (t, t.contiguous(memory_format=torch.channels_last), t[:2], t.permute(2, 0, 3, 1), t[:, :1, :1, :1][:1], torch.zeros(())):
+        assert ops._dense_run(v)
+    for v in (t[:, :2], t[..., ::2], t[:1].expand(5, 6, 3, 3), torch.zeros(8)[::2]):
+        assert not ops._dense_run(v)
+
+
+@pytest.mark.parametrize("segments", [[(0, 5, 0)], [(3, 4096, 1), (4099, 10_000, 0)], [(8, 0, 0), (8, 9000, 1)], [(20_000, 7, 0), (0, 9, 1)]],
+                         ids=str)
+def test_step_table_covers_each_element_once(segments):
+    t = ops.sgd_clip_table(segments, "cpu")
+    got = {}
+    for first, count, group, tensor in t.blocks.tolist():
+        assert 0 < count <= 4096 and segments[tensor][2] == group
+        for i in range(first, first + count):
+            assert i not in got
+            got[i] = tensor
+    want = {i: k for k, (a, n, _) in enumerate(segments) for i in range(a, a + n)}
+    assert got == want and t.n_blocks == len(t.blocks) and t.end == max(want) + 1 and t.n_tensors == len(segments)
+
+
+def test_step_table_refusals():
+    for bad in ([], [(0, 0, 0)], [(0, 5, 2)], [(-1, 5, 0)], [(0, 5, 0), (4, 2, 1)], [(0, 1 << 31, 0)]):
+        with pytest.raises(ValueError):
+            ops.sgd_clip_table(bad, "cpu")
+
+
+def test_clip_settings():
+    from yolo_amd.config import get_cfg
+    cfg = get_cfg()
+    assert cfg.SOLVER.CLIP_GRADIENTS.ENABLED is False and cfg.SOLVER.CLIP_GRADIENTS.CLIP_TYPE == "value"
+    model = torch.nn.Sequential(torch.nn.Linear(3, 2))
+    assert solver.build_optimizer(cfg, model)._clip is None
+    cfg.merge_from_list(["SOLVER.CLIP_GRADIENTS.ENABLED", True, "SOLVER.CLIP_GRADIENTS.CLIP_TYPE", "full_model",
+                         "SOLVER.CLIP_GRADIENTS.CLIP_VALUE", 10.0])
+    opt = solver.build_optimizer(cfg, model)
+    assert opt._clip == ("full_model", 10.0, 2.0)
+    opt.step()                     # no gradients: nothing to clip
+    with pytest.raises(RuntimeError, match="closure"):
+        opt.step(lambda: 0.0)
+    model[0].weight.grad = torch.ones(2, 3)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        opt.step()
+    for key, value in (("CLIP_TYPE", "each"), ("CLIP_VALUE", -1.0), ("NORM_TYPE", 3.0)):
+        c = cfg.clone()
+        c.merge_from_list([f"SOLVER.CLIP_GRADIENTS.{key}", value])
+        with pytest.raises(ValueError):
+            solver.build_optimizer(c, model)
+    assert float(solver.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0)) == 0.0

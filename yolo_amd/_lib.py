@@ -106,6 +106,18 @@ SIGNATURES = {
     "yolo_aug_resample_batch": (c_int, [c_void_p, c_int, c_void_p]),
     "yolo_sgd_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_float, c_float, c_float, c_float,
                               c_void_p]),
+    "yolo_gn_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "yolo_gn_act_fwd": (c_int, [_VP, c_void_p, c_void_p, _VP, _VP, c_void_p, c_int, c_int, c_int, c_float, c_int, c_float,
+                                c_int, c_void_p, c_size_t, c_void_p]),
+    "yolo_gn_act_bwd": (c_int, [_VP, _VP, c_void_p, c_void_p, c_void_p, _VP, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                                c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "yolo_grad_norm_workspace_bytes": (c_size_t, [c_int]),
+    "yolo_grad_norm": (c_int, [c_void_p, c_int, c_void_p, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p, c_size_t,
+                               c_void_p]),
+    "yolo_grad_scale": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p]),
+    "yolo_grad_clamp": (c_int, [c_void_p, c_int, c_float, c_void_p]),
+    "yolo_sgd_step_clipped": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_float, c_float, c_float,
+                                      c_float, c_void_p, c_int, c_float, c_void_p]),
     "yolo_conv3x3s2_dgrad": (c_int, [_VP, c_void_p, c_void_p, _VP, _VP, c_int, c_int, c_int, c_int, c_void_p]),
     "yolo_pack_conv_train_batch": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p]),
     "yolo_pack_conv_train": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int,

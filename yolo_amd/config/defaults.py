@@ -67,6 +67,11 @@ _C.SOLVER.WARMUP_METHOD = "linear"
 _C.SOLVER.CHECKPOINT_PERIOD = 5000
 _C.SOLVER.IMS_PER_BATCH = 16
 _C.SOLVER.REFERENCE_WORLD_SIZE = 0
+_C.SOLVER.CLIP_GRADIENTS = CN()
+_C.SOLVER.CLIP_GRADIENTS.ENABLED = False
+_C.SOLVER.CLIP_GRADIENTS.CLIP_TYPE = "value"     # "value", "norm" (each tensor), "full_model" (all tensors together)
+_C.SOLVER.CLIP_GRADIENTS.CLIP_VALUE = 1.0
+_C.SOLVER.CLIP_GRADIENTS.NORM_TYPE = 2.0         # 1, 2 or inf
 
 _C.TEST = CN()
 _C.TEST.EVAL_PERIOD = 0

@@ -17,6 +17,7 @@ from ._lib import YoloView, check, lib
 
 F32, BF16 = 0, 1
 NMS_PER_CLASS, NMS_COORD_TRICK, NMS_AUTO = 0, 1, 2
+ACTIVATIONS = {"leaky": 0, "silu": 1}
 
 
 def dtype_code(dt: torch.dtype) -> int:
@@ -436,6 +437,66 @@ def bn_act_bwd(dy: View, z: View, stats: torch.Tensor, dz: View, dgamma: torch.T
     check(lib().yolo_bn_act_bwd(ctypes.byref(dyv), ctypes.byref(zv), _ptr(stats), ctypes.byref(dzv), z.N, z.C,
                                 float(slope), dtype_code(z.buf.dtype), _ptr(dgamma), _ptr(dbeta), _ptr(workspace),
                                 workspace.numel() * workspace.element_size(), _stream()), "yolo_bn_act_bwd")
+
+
+def gn_workspace_bytes(N: int, H: int, W: int, C: int, groups: int, dtype: torch.dtype) -> int:
+    """Bytes of workspace gn_act_fwd and gn_act_bwd take (one buffer serves both, one call at a time)."""
+    return int(lib().yolo_gn_workspace_bytes(N, H, W, C, groups, dtype_code(dtype)))
+
+
+def _check_gn(what: str, views, vectors, stats: torch.Tensor, workspace: torch.Tensor, groups: int, act: str) -> None:
+    first = views[0][1]
+    for name, v in views:
+        _require_cuda(v.buf, f"{what}: {name}")
+        # the kernels address the view from its struct alone: the buffer behind it has to be what the struct says
+        if not v.buf.is_contiguous() or v.buf.dim() != 4 or v.buf.shape[1] != v.H + 2 * v.halo or v.buf.shape[2] != v.W + 2 * v.halo:
+            raise ValueError(f"{what}: {name}: a {v.H} x {v.W} view with halo {v.halo} does not describe its "
+                             f"{tuple(v.buf.shape)} buffer")
+        if v.buf.dtype != first.buf.dtype or (v.N, v.C) != (first.N, first.C):
+            raise ValueError(f"{what}: {name} is {v.N} x {v.C} channels of {v.buf.dtype}, expected {first.N} x {first.C} of "
+                             f"{first.buf.dtype}")
+    for name, t in vectors:
+        _require_cuda(t, f"{what}: {name}")
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != first.C:
+            raise ValueError(f"{what}: {name} has to be a contiguous float32 vector of {first.C}")
+    _require_cuda(stats, f"{what}: stats")
+    if stats.dtype != torch.float32 or not stats.is_contiguous() or stats.numel() != 2 * first.N * groups:
+        raise ValueError(f"{what}: stats has to be a contiguous float32 tensor [2, {first.N}, {groups}]")
+    _require_cuda(workspace, f"{what}: workspace")
+    if not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace has to be contiguous")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"{what}: activation {act!r} (one of {', '.join(ACTIVATIONS)})")
+
+
+def gn_act_fwd(x: View, gamma: torch.Tensor, beta: torch.Tensor, y: View, stats: torch.Tensor, workspace: torch.Tensor, *,
+               groups: int, eps: float = 1e-5, act: str = "leaky", slope: float = 0.1,
+               residual: Optional[View] = None) -> None:
+    """y = act(group_norm(x) * gamma + beta) [+ residual]; stats [2, N, groups] f32 <- mean and 1 / sqrt(var + eps), for
+    gn_act_bwd.  ``act``: "leaky" with ``slope`` in [0, 1] (1: no activation, 0: ReLU) or "silu".  ``y`` may be ``x`` or
+    ``residual`` (each element is read before it is written); f32 or bf16, sums in f32 / f64."""
+    _check_gn("gn_act_fwd", [("x", x), ("y", y)] + ([("residual", residual)] if residual is not None else []),
+              [("gamma", gamma), ("beta", beta)], stats, workspace, groups, act)
+    xv, yv = x.c(), y.c()
+    rv = residual.c() if residual is not None else None
+    check(lib().yolo_gn_act_fwd(ctypes.byref(xv), _ptr(gamma), _ptr(beta), ctypes.byref(rv) if rv is not None else None,
+                                ctypes.byref(yv), _ptr(stats), x.N, x.C, groups, float(eps), ACTIVATIONS[act], float(slope),
+                                dtype_code(x.buf.dtype), _ptr(workspace), workspace.numel() * workspace.element_size(),
+                                _stream()), "yolo_gn_act_fwd")
+
+
+def gn_act_bwd(dy: View, x: View, gamma: torch.Tensor, beta: torch.Tensor, stats: torch.Tensor, dx: View,
+               dgamma: torch.Tensor, dbeta: torch.Tensor, workspace: torch.Tensor, *, groups: int, act: str = "leaky",
+               slope: float = 0.1) -> None:
+    """Backward of gn_act_fwd from its input and ``stats``: dx, dgamma [C], dbeta [C] (f32, overwritten).  The residual's
+    gradient is dy itself.  ``dx`` may be ``dy`` or ``x``."""
+    _check_gn("gn_act_bwd", [("x", x), ("dy", dy), ("dx", dx)],
+              [("gamma", gamma), ("beta", beta), ("dgamma", dgamma), ("dbeta", dbeta)], stats, workspace, groups, act)
+    dyv, xv, dxv = dy.c(), x.c(), dx.c()
+    check(lib().yolo_gn_act_bwd(ctypes.byref(dyv), ctypes.byref(xv), _ptr(gamma), _ptr(beta), _ptr(stats), ctypes.byref(dxv),
+                                _ptr(dgamma), _ptr(dbeta), x.N, x.C, groups, ACTIVATIONS[act], float(slope),
+                                dtype_code(x.buf.dtype), _ptr(workspace), workspace.numel() * workspace.element_size(),
+                                _stream()), "yolo_gn_act_bwd")
 
 
 def wgrad_workspace_bytes(M: int, cin: int, cout: int, k: int) -> int:
@@ -867,3 +928,151 @@ def sgd_step(param: torch.Tensor, grad: torch.Tensor, mom: torch.Tensor, table: 
     assert param.dtype == grad.dtype == mom.dtype == torch.float32 and param.numel() == grad.numel() == mom.numel()
     check(lib().yolo_sgd_step(_ptr(param), _ptr(grad), _ptr(mom), _ptr(table), n_blocks, lr0, wd0, lr1, wd1, momentum,
                               _stream()), "yolo_sgd_step")
+
+
+# ---------------------------------------------------------------------------------------------------------
+# gradient norms and clipping
+# ---------------------------------------------------------------------------------------------------------
+class GradBlock(ctypes.Structure):
+    """yolo_grad_block of include/yolo_hip.h."""
+    _fields_ = [("ptr", ctypes.c_void_p), ("count", ctypes.c_int), ("tensor", ctypes.c_int), ("dtype", ctypes.c_int),
+                ("reserved", ctypes.c_int)]
+
+
+@dataclass
+class GradTable:
+    """Which elements of which tensors the gradient operators work on (``grad_table``): the tensors must stay in place for as
+    long as the table is used (it keeps them alive)."""
+    blocks: torch.Tensor     # device, n_blocks yolo_grad_block
+    n_blocks: int
+    first: torch.Tensor      # device, [n_tensors + 1] int32: a tensor's first block
+    tensors: list
+
+    @property
+    def n_tensors(self) -> int:
+        return len(self.tensors)
+
+
+def _dense_run(t: torch.Tensor) -> bool:
+    """Whether the tensor's elements are one run of memory in some order of its dimensions (a channels_last weight is)."""
+    expected = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda p: p[1]):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def grad_table(tensors: Sequence[torch.Tensor]) -> GradTable:
+    """Table of ``tensors`` (float32 or bfloat16, each one run of memory in some dimension order, none twice) for grad_norm,
+    grad_scale and grad_clamp.  Built on the host and copied once: build it outside graph capture."""
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError("grad_table: no tensors")
+    for t in tensors:
+        _require_cuda(t, "grad_table")
+        dtype_code(t.dtype)
+        if t.numel() and not _dense_run(t):
+            raise ValueError(f"grad_table: a tensor {tuple(t.shape)} with strides {tuple(t.stride())} is not one run of memory")
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError("grad_table: two tensors share memory (a shared gradient is listed once)")
+    # runs of a workgroup: 16384 elements, shorter where the whole set would not give each CU eight
+    total = sum(t.numel() for t in tensors)
+    run = max(1024, min(16384, -(-total // 2048) // 1024 * 1024))
+    rows, first = [], [0]
+    for i, t in enumerate(tensors):
+        n, es = t.numel(), t.element_size()
+        rows += [(t.data_ptr() + o * es, min(run, n - o), i, dtype_code(t.dtype), 0) for o in range(0, n, run)]
+        first.append(len(rows))
+    dev = tensors[0].device
+    raw = (GradBlock * max(1, len(rows)))(*rows)
+    blocks = torch.frombuffer(bytearray(bytes(raw)), dtype=torch.uint8).to(dev)
+    return GradTable(blocks, len(rows), torch.tensor(first, dtype=torch.int32).to(dev), tensors)
+
+
+def grad_norm_workspace_bytes(table: GradTable) -> int:
+    return int(lib().yolo_grad_norm_workspace_bytes(table.n_blocks))
+
+
+def _check_norms(t: Optional[torch.Tensor], n: int, what: str) -> None:
+    if t is None:
+        return
+    _require_cuda(t, what)
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n:
+        raise ValueError(f"{what}: expected a contiguous float32 tensor of {n}")
+
+
+def grad_norm(table: GradTable, norms: torch.Tensor, workspace: torch.Tensor, *, norm_type: float = 2.0,
+              per_tensor: bool = False, max_norm: float = 0.0, coefs: Optional[torch.Tensor] = None) -> None:
+    """norms [1] <- the norm (1, 2 or inf) of all the table's tensors together, or [n_tensors] <- of each; coefs, of the same
+    length, <- min(1, max_norm / (norm + 1e-6)).  Nothing is read back to the host."""
+    _require_cuda(table.blocks, "grad_norm")
+    n = table.n_tensors if per_tensor else 1
+    _check_norms(norms, n, "grad_norm: norms")
+    _check_norms(coefs, n, "grad_norm: coefs")
+    _require_cuda(workspace, "grad_norm: workspace")
+    check(lib().yolo_grad_norm(_ptr(table.blocks), table.n_blocks, _ptr(table.first) if per_tensor else None,
+                               table.n_tensors, float(norm_type), float(max_norm), _ptr(norms), _ptr(coefs), _ptr(workspace),
+                               workspace.numel() * workspace.element_size(), _stream()), "yolo_grad_norm")
+
+
+def grad_scale(table: GradTable, coefs: torch.Tensor, *, per_tensor: bool = False) -> None:
+    """Multiply the table's tensors by coefs [1], or each by its own of coefs [n_tensors], in place."""
+    _require_cuda(table.blocks, "grad_scale")
+    _check_norms(coefs, table.n_tensors if per_tensor else 1, "grad_scale: coefs")
+    check(lib().yolo_grad_scale(_ptr(table.blocks), table.n_blocks, _ptr(coefs), int(per_tensor), _stream()), "yolo_grad_scale")
+
+
+def grad_clamp(table: GradTable, value: float) -> None:
+    """Clamp the table's tensors to [-value, value] in place."""
+    _require_cuda(table.blocks, "grad_clamp")
+    check(lib().yolo_grad_clamp(_ptr(table.blocks), table.n_blocks, float(value), _stream()), "yolo_grad_clamp")
+
+
+@dataclass
+class SgdClipTable:
+    """Which runs of the arenas sgd_step_clipped's workgroups own (``sgd_clip_table``)."""
+    blocks: torch.Tensor     # device, [n_blocks, 4] int32: first element, count, group, tensor
+    n_blocks: int
+    n_tensors: int
+    end: int                 # one past the last element any run covers
+
+
+def sgd_clip_table(segments: Sequence[Tuple[int, int, int]], device) -> SgdClipTable:
+    """Block table of ``sgd_step_clipped`` for ``segments`` = (first element, count, group) runs of the arenas, one for each
+    tensor in the order of the clip factors; no element is in two of them."""
+    rows, spans = [], []
+    for tensor, (first, count, group) in enumerate(segments):
+        if first < 0 or count < 0 or group not in (0, 1) or first + count >= 1 << 31:
+            raise ValueError(f"sgd_clip_table: segment ({first}, {count}, {group})")
+        spans.append((first, first + count))
+        at, end = first, first + count
+        while at < end:   # runs end at multiples of 4096 elements, so that all but a segment's first begin aligned
+            n = min(end, (at // 4096 + 1) * 4096) - at
+            rows.append((at, n, group, tensor))
+            at += n
+    spans = sorted(s for s in spans if s[0] < s[1])
+    if not spans or any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError("sgd_clip_table: no elements, or an element in two segments")
+    return SgdClipTable(torch.tensor(rows, dtype=torch.int32, device=device).contiguous(), len(rows), len(segments), spans[-1][1])
+
+
+def sgd_step_clipped(param: torch.Tensor, grad: torch.Tensor, mom: torch.Tensor, table: SgdClipTable, lr0: float, wd0: float,
+                     lr1: float, wd1: float, momentum: float, *, coefs: Optional[torch.Tensor] = None,
+                     per_tensor: bool = False, clip_value: Optional[float] = None) -> None:
+    """sgd_step on clipped gradients, in the same one launch: grad times coefs [1] (or the factor of its tensor), or clamped to
+    [-clip_value, clip_value].  ``grad`` itself is left as it is."""
+    for what, t in (("param", param), ("grad", grad), ("mom", mom)):
+        _require_cuda(t, f"sgd_step_clipped: {what}")
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != param.numel():
+            raise ValueError(f"sgd_step_clipped: {what} has to be a contiguous float32 arena of {param.numel()} elements")
+    if (coefs is None) == (clip_value is None):
+        raise ValueError("sgd_step_clipped: give coefs or clip_value, one of the two")
+    _require_cuda(table.blocks, "sgd_step_clipped: table")
+    if table.end > param.numel():
+        raise ValueError(f"sgd_step_clipped: the table covers {table.end} elements, the arenas have {param.numel()}")
+    _check_norms(coefs, table.n_tensors if per_tensor else 1, "sgd_step_clipped: coefs")
+    check(lib().yolo_sgd_step_clipped(_ptr(param), _ptr(grad), _ptr(mom), _ptr(table.blocks), table.n_blocks, lr0, wd0, lr1, wd1,
+                                      momentum, _ptr(coefs), int(per_tensor), -1.0 if clip_value is None else float(clip_value),
+                                      _stream()), "yolo_sgd_step_clipped")
