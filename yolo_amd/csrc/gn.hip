@@ -26,6 +26,9 @@ struct GnParams {
     int N, H, W, HW, C, Cg, groups;
     int VS, PL;            // 16-byte vectors of a slab, pixel lanes of a workgroup
     int chunk, chunks;     // pixels of a workgroup, workgroups of an image's slab
+    int slabs;             // whole-image kernels: slabs of an image
+    int stream;            // the call moves more than the caches hold: loads and stores that do not stay in them
+    int fold;              // whole-image kernel: channels folded in a thread (a power of two dividing Cg)
     const float* gamma;
     const float* beta;
     float* stats;          // [2][N][groups]: mean, r
@@ -66,25 +69,67 @@ template <> struct GnVec<float> {
     }
 };
 
-// A position in an image, moved on by a fixed number of pixels without divisions.
+// K channels of a vector, the ones from part * K on.
+template <typename E, int K>
+__device__ __forceinline__ void gn_part(const u32x4& r, int part, float* v) {
+    if constexpr (sizeof(E) == 2 && K == 4) {
+        v[0] = __uint_as_float(r[2 * part] << 16);
+        v[1] = __uint_as_float(r[2 * part] & 0xffff0000u);
+        v[2] = __uint_as_float(r[2 * part + 1] << 16);
+        v[3] = __uint_as_float(r[2 * part + 1] & 0xffff0000u);
+    } else {
+        GnVec<E>::unpack(r, v);
+    }
+}
+
+// Byte offsets of a pixel's vector from the image's start in K tensors (below 2^31: the host checks), moved on by a fixed number
+// of pixels without divisions or products.
+template <int K>
 struct GnCursor {
-    int h, w, sh, sw, W;
-    __device__ __forceinline__ GnCursor(int pixel, int step, int W_) : W(W_) {
-        h = pixel / W;
+    int w, sw, W;
+    int at[K], step[K], wrap[K];
+    __device__ __forceinline__ GnCursor(int pixel, int pixels, int W_, int cb, const GnTensor* const (&t)[K]) : W(W_) {
+        const int h = pixel / W, sh = pixels / W;
         w = pixel - h * W;
-        sh = step / W;
-        sw = step - sh * W;
+        sw = pixels - sh * W;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            at[k] = h * t[k]->row + w * t[k]->pix + cb;
+            step[k] = sh * t[k]->row + sw * t[k]->pix;
+            wrap[k] = t[k]->row - W * t[k]->pix;
+        }
     }
     __device__ __forceinline__ void next() {
         w += sw;
-        h += sh;
-        if (w >= W) {
-            w -= W;
-            ++h;
-        }
+        const bool over = w >= W;
+        w -= over ? W : 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) at[k] += step[k] + (over ? wrap[k] : 0);
     }
-    __device__ __forceinline__ int at(const GnTensor& t) const { return h * t.row + w * t.pix; }
 };
+
+// ST: a load of what is not read again soon, a store that leaves the caches to what is.  `base` is uniform, the offset a thread's.
+template <int ST = 0>
+__device__ __forceinline__ u32x4 gn_load(const char* base, unsigned at) {
+    if constexpr (ST) return __builtin_nontemporal_load((const u32x4*)(base + at));
+    return *(const u32x4*)(base + at);
+}
+template <int ST>
+__device__ __forceinline__ void gn_store(char* base, unsigned at, const u32x4& v) {
+    if constexpr (ST)
+        __builtin_nontemporal_store(v, (u32x4*)(base + at));
+    else
+        *(u32x4*)(base + at) = v;
+}
+template <int N> struct GnCount { static constexpr int value = N; };
+// f with the call's kind of loads and stores
+template <typename F>
+__device__ __forceinline__ void gn_with_stream(int stream, F f) {
+    if (stream)
+        f(GnCount<1>{});
+    else
+        f(GnCount<0>{});
+}
 
 constexpr int GN_LEAKY = YOLO_ACT_LEAKY, GN_SILU = YOLO_ACT_SILU;
 
@@ -98,21 +143,132 @@ __device__ __forceinline__ float gn_act(float t, float slope) {
     return t > 0.f ? t : t * slope;
 }
 
-// d = dy * act'(t) with t = xh * gamma + beta.  The leaky derivative jumps at t = 0 (slope at t == 0, torch's convention), so
-// the side is decided exactly: fp32 rounds t by less than 2^-22 (|beta| + |t|) -- three roundings of xh * gamma, which is
-// about -beta there, and one of the sum -- and a t nearer to zero than 2^-20 |beta| is computed again in fp64.  One value in
-// about a million takes that branch.
+// d = dy * act'(t); `least` keeps the smallest |t| seen.  The leaky derivative jumps at t = 0 (slope at t == 0, torch's
+// convention), and its side is decided exactly.  t = (x - mean) * (gamma r) + beta in fp32 is off by less than 2^-22 (|beta| +
+// |t|): two roundings in each factor's product, which is about -beta where t is small, and one of the sum.  Where `least` ends
+// up below 2^-20 times the largest |beta| of the channels (gn_near) -- one vector in some hundred thousand -- their values are
+// done again with the sides from fp64 (gn_exact_side).
 template <int ACT>
-__device__ __forceinline__ float gn_act_grad(float dy, float x, float xh, float mean, float r, float gamma, float beta, float slope) {
-    const float t = xh * gamma + beta;
+__device__ __forceinline__ float gn_act_grad(float dy, float t, float slope, float& least) {
     if constexpr (ACT == GN_SILU) {
         const float s = gn_sigmoid(t);
         return dy * (s * (1.f + t * (1.f - s)));
     } else {
-        bool up = t > 0.f;
-        if (__builtin_expect(fabsf(t) <= fabsf(beta) * 0x1p-20f, 0))
-            up = ((double)x - (double)mean) * (double)r * (double)gamma + (double)beta > 0.0;
-        return up ? dy : dy * slope;
+        least = fminf(least, fabsf(t));
+        return dy * (t > 0.f ? 1.f : slope);
+    }
+}
+// 1 where t > 0 and slope elsewhere, from the channel's constants in LDS: {mean, r, gamma, beta}, `row` floats apart, at `c`.  The
+// index is opaque and one call ends before the next one begins: the loops around the calls need the registers that constants
+// loaded ahead would take.
+__device__ __forceinline__ float gn_exact_side(float x, const float* lds, int c, int row, float slope) {
+    asm volatile("" : "+v"(c));
+    float side = ((double)x - (double)lds[c]) * (double)lds[c + row] * (double)lds[c + 2 * row] + (double)lds[c + 3 * row] > 0.0 ? 1.f : slope;
+    asm volatile("" : "+v"(side));
+    return side;
+}
+template <int K>
+__device__ __forceinline__ float gn_near(const float* beta) {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < K; ++e) m = fmaxf(m, fabsf(beta[e]));
+    return m * 0x1p-20f;
+}
+
+// The constants of a slab's channels in LDS: {mean, r, gamma, beta}, S floats each.
+__device__ __forceinline__ void gn_stage(float* k, const GnParams& p, int n, int c0, int S) {
+    for (int j = threadIdx.x; j < S && c0 + j < p.C; j += GN_THREADS) {
+        const int g = (c0 + j) / p.Cg;
+        k[j] = p.stats[n * p.groups + g];
+        k[S + j] = p.stats[(p.N + n) * p.groups + g];
+        k[2 * S + j] = p.gamma[c0 + j];
+        k[3 * S + j] = p.beta[c0 + j];
+    }
+    __syncthreads();
+}
+// Makes the compiler forget what it has unpacked from the vectors, and loaded so far: kept between two passes it would not fit.
+template <int NV>
+__device__ __forceinline__ void gn_forget(u32x4 (&v)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i])::"memory");
+}
+
+// What a thread needs of its V channels: t = (x - mean) * scale + beta with scale = gamma * r.
+template <int V>
+struct GnConst {
+    float mean[V], scale[V], beta[V];
+    __device__ __forceinline__ GnConst(const float* k, int S) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            mean[e] = k[e];
+            scale[e] = k[2 * S + e] * k[S + e];
+            beta[e] = k[3 * S + e];
+        }
+    }
+};
+
+// x - mean and d = dy * act'(t) of a vector's channels; k holds the constants of K of them, the ones from `part` * K on.
+template <typename E, int ACT, int K>
+__device__ __forceinline__ void gn_grads_of(const u32x4& x, const u32x4& dy, int part, const GnConst<K>& k, float near, const float* lds, int c,
+                                            int row, float slope, float* xm, float* a) {
+    float least = INFINITY;
+    gn_part<E, K>(x, part, xm);
+    gn_part<E, K>(dy, part, a);
+#pragma unroll
+    for (int e = 0; e < K; ++e) {
+        xm[e] -= k.mean[e];
+        a[e] = gn_act_grad<ACT>(a[e], fmaf(xm[e], k.scale[e], k.beta[e]), slope, least);
+    }
+    if (ACT == GN_LEAKY && __builtin_expect(least <= near, 0)) {
+        u32x4 again[2] = {x, dy};
+        gn_forget<2>(again);
+        float v[K];
+        gn_part<E, K>(again[0], part, v);
+        gn_part<E, K>(again[1], part, a);
+#pragma unroll
+        for (int e = 0; e < K; ++e) a[e] *= gn_exact_side(v[e], lds, c + e, row, slope);
+    }
+}
+template <typename E, int ACT>
+__device__ __forceinline__ void gn_grads(const u32x4& x, const u32x4& dy, const GnConst<GnVec<E>::N>& k, float near, const float* lds, int c,
+                                         int row, float slope, float* xm, float* a) {
+    gn_grads_of<E, ACT, GnVec<E>::N>(x, dy, 0, k, near, lds, c, row, slope, xm, a);
+}
+
+// count steps, four at a time (their loads are all issued before the first is used), then one at a time.
+template <typename F>
+__device__ __forceinline__ void gn_in_fours(int count, F f) {
+    int i = 0;
+    for (; i + 4 <= count; i += 4) f(GnCount<4>{});
+    for (; i < count; ++i) f(GnCount<1>{});
+}
+
+// count steps, U at a time: the loads of the next U are on their way while the last U are used.  load(r) takes the next step's
+// vectors, use(r) uses them.
+template <int U, int K, typename L, typename F>
+__device__ __forceinline__ void gn_pipelined(int count, L load, F use) {
+    u32x4 now[U][K];
+    int i = 0;
+    if (count >= U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(now[u]);
+        for (i = U; i + U <= count; i += U) {
+            u32x4 next[U][K];
+#pragma unroll
+            for (int u = 0; u < U; ++u) load(next[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) use(now[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < K; ++k) now[u][k] = next[u][k];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) use(now[u]);
+    }
+    for (; i < count; ++i) {
+        load(now[0]);
+        use(now[0]);
     }
 }
 
@@ -135,33 +291,38 @@ __device__ __forceinline__ GnLane gn_lane(const GnParams& p) {
 // partial[n][chunk][0 / 1][c] = sum of x, of x * x over the chunk's pixels.  A thread sums differences from the first value
 // it sees (fp32; the values of a few dozen pixels differ from it by about their spread), and goes over to fp64 after that.
 template <typename E>
-__global__ void __launch_bounds__(GN_THREADS) gn_sums_kernel(const GnParams p) {
+__global__ void __launch_bounds__(GN_THREADS, 5) gn_sums_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
     __shared__ double red[GN_THREADS * V];
     const GnLane l = gn_lane<E>(p);
     const int n = blockIdx.z, first = blockIdx.x * p.chunk, last = min(first + p.chunk, p.HW);
-    const char* base = p.x.p + n * p.x.img + l.c * (int)sizeof(E);
+    const char* base = p.x.p + n * p.x.img;
+    const int cb = l.c * (int)sizeof(E);
     float k[V], s[V], q[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) k[e] = s[e] = q[e] = 0.f;
     int count = 0;
     if (l.on && first + l.pl < last) {
-        GnCursor c(first + l.pl, p.PL, p.W);
+        GnCursor<1> c(first + l.pl, p.PL, p.W, cb, {&p.x});
         count = (last - first - l.pl + p.PL - 1) / p.PL;
-        GnVec<E>::unpack(*(const u32x4*)(base + c.at(p.x)), k);
+        GnVec<E>::unpack(gn_load(base, c.at[0]), k);
         c.next();
-#pragma unroll 4
-        for (int i = 1; i < count; ++i) {
-            float v[V];
-            GnVec<E>::unpack(*(const u32x4*)(base + c.at(p.x)), v);
-            c.next();
+        gn_pipelined<4, 1>(
+            count - 1,
+            [&](u32x4* r) {
+                r[0] = gn_load(base, c.at[0]);
+                c.next();
+            },
+            [&](const u32x4* r) {
+                float v[V];
+                GnVec<E>::unpack(r[0], v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float d = v[e] - k[e];
-                s[e] += d;
-                q[e] += d * d;
-            }
-        }
+                for (int e = 0; e < V; ++e) {
+                    const float d = v[e] - k[e];
+                    s[e] += d;
+                    q[e] = fmaf(d, d, q[e]);
+                }
+            });
     }
     const int S = p.VS * V;
     double* out = (double*)p.partial + (((long long)n * p.chunks + blockIdx.x) * 2) * p.C + blockIdx.y * S;
@@ -206,101 +367,118 @@ __global__ void __launch_bounds__(64) gn_stats_kernel(const GnParams p) {
 
 // ------------------------------------------------------------------------------------------------ forward, output
 template <typename E, int ACT>
-__global__ void __launch_bounds__(GN_THREADS) gn_apply_kernel(const GnParams p) {
+__global__ void __launch_bounds__(GN_THREADS, 8) gn_apply_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
+    // fp32: (x - mean) * scale + beta; bf16: x * scale + (beta - mean * scale), whose rounding of mean * scale is far below the
+    // output's
+    constexpr bool SHIFT = sizeof(E) == 2;
     const GnLane l = gn_lane<E>(p);
     // the pass before this one walked forwards: its last chunks are the ones still in the caches
     const int n = p.N - 1 - blockIdx.z, chunk = p.chunks - 1 - blockIdx.x;
     const int first = chunk * p.chunk, last = min(first + p.chunk, p.HW);
     if (!l.on || first + l.pl >= last) return;
-    float mean[V], sc[V], beta[V];
+    float mean[V], scale[V], shift[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int g = (l.c + e) / p.Cg;
         mean[e] = p.stats[n * p.groups + g];
-        sc[e] = p.gamma[l.c + e] * p.stats[(p.N + n) * p.groups + g];
-        beta[e] = p.beta[l.c + e];
+        scale[e] = p.gamma[l.c + e] * p.stats[(p.N + n) * p.groups + g];
+        shift[e] = SHIFT ? fmaf(-mean[e], scale[e], p.beta[l.c + e]) : p.beta[l.c + e];
     }
     const int cb = l.c * (int)sizeof(E);
-    const char* x = p.x.p + n * p.x.img + cb;
-    const char* r = p.r.p ? p.r.p + n * p.r.img + cb : nullptr;
-    char* y = p.y.p + n * p.y.img + cb;
+    const char* x = p.x.p + n * p.x.img;
+    char* y = p.y.p + n * p.y.img;
     const int count = (last - first - l.pl + p.PL - 1) / p.PL;
-    GnCursor c(first + l.pl, p.PL, p.W);
+    gn_with_stream(p.stream, [&](auto st) {
+        constexpr int ST = decltype(st)::value;
+        auto put = [&](const u32x4& raw, const u32x4* res, unsigned to) {
+            float v[V];
+            GnVec<E>::unpack(raw, v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = gn_act<ACT>(fmaf(SHIFT ? v[e] : v[e] - mean[e], scale[e], shift[e]), p.slope);
+            if (res) {
+                float a[V];
+                GnVec<E>::unpack(*res, a);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] += a[e];
+            }
+            gn_store<ST>(y, to, GnVec<E>::pack(v));
+        };
+        if (p.r.p) {
+            const char* r = p.r.p + n * p.r.img;
+            GnCursor<3> c(first + l.pl, p.PL, p.W, cb, {&p.x, &p.r, &p.y});
 #pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-        float v[V];
-        GnVec<E>::unpack(*(const u32x4*)(x + c.at(p.x)), v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = gn_act<ACT>((v[e] - mean[e]) * sc[e] + beta[e], p.slope);
-        if (r) {
-            float a[V];
-            GnVec<E>::unpack(*(const u32x4*)(r + c.at(p.r)), a);
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] += a[e];
+            for (int i = 0; i < count; ++i) {
+                const u32x4 res = gn_load<ST>(r, c.at[1]);
+                put(gn_load<ST>(x, c.at[0]), &res, c.at[2]);
+                c.next();
+            }
+        } else {
+            GnCursor<2> c(first + l.pl, p.PL, p.W, cb, {&p.x, &p.y});
+#pragma unroll 4
+            for (int i = 0; i < count; ++i) {
+                put(gn_load<ST>(x, c.at[0]), nullptr, c.at[1]);
+                c.next();
+            }
         }
-        *(u32x4*)(y + c.at(p.y)) = GnVec<E>::pack(v);
-        c.next();
-    }
+    });
 }
 
 // ------------------------------------------------------------------------------------------------ backward, sums
 // partial[n][chunk][0 / 1][c] = sum of d, of d * xh over the chunk's pixels
 template <typename E, int ACT>
-__global__ void __launch_bounds__(GN_THREADS) gn_bwd_sums_kernel(const GnParams p) {
+__global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_sums_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
-    __shared__ float red[2][GN_THREADS * V];
+    __shared__ __attribute__((aligned(16))) float lds[4 * GN_THREADS * V];  // the slab's constants, then its threads' sums
     const GnLane l = gn_lane<E>(p);
-    const int n = blockIdx.z, first = blockIdx.x * p.chunk, last = min(first + p.chunk, p.HW);
+    const int n = blockIdx.z, first = blockIdx.x * p.chunk, last = min(first + p.chunk, p.HW), S = p.VS * V;
+    const float* mine = lds + (l.c - blockIdx.y * S);
+    gn_stage(lds, p, n, blockIdx.y * S, S);
     float sd[V], sx[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) sd[e] = sx[e] = 0.f;
     if (l.on && first + l.pl < last) {
-        float mean[V], is[V], gamma[V], beta[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const int g = (l.c + e) / p.Cg;
-            mean[e] = p.stats[n * p.groups + g];
-            is[e] = p.stats[(p.N + n) * p.groups + g];
-            gamma[e] = p.gamma[l.c + e];
-            beta[e] = p.beta[l.c + e];
-        }
+        const GnConst<V> k(mine, S);
         const int cb = l.c * (int)sizeof(E);
-        const char* x = p.x.p + n * p.x.img + cb;
-        const char* dy = p.dy.p + n * p.dy.img + cb;
+        const char* x = p.x.p + n * p.x.img;
+        const char* dy = p.dy.p + n * p.dy.img;
         const int count = (last - first - l.pl + p.PL - 1) / p.PL;
-        GnCursor c(first + l.pl, p.PL, p.W);
-#pragma unroll 4
-        for (int i = 0; i < count; ++i) {
-            float v[V], d[V];
-            GnVec<E>::unpack(*(const u32x4*)(x + c.at(p.x)), v);
-            GnVec<E>::unpack(*(const u32x4*)(dy + c.at(p.dy)), d);
-            c.next();
+        const float near = gn_near<V>(k.beta);
+        GnCursor<2> c(first + l.pl, p.PL, p.W, cb, {&p.x, &p.dy});
+        gn_pipelined<2, 2>(
+            count,
+            [&](u32x4* r) {
+                r[0] = gn_load(x, c.at[0]);
+                r[1] = gn_load(dy, c.at[1]);
+                c.next();
+            },
+            [&](const u32x4* r) {
+                float xm[V], a[V];
+                gn_grads<E, ACT>(r[0], r[1], k, near, lds, l.c - blockIdx.y * S, S, p.slope, xm, a);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float xh = (v[e] - mean[e]) * is[e];
-                const float a = gn_act_grad<ACT>(d[e], v[e], xh, mean[e], is[e], gamma[e], beta[e], p.slope);
-                sd[e] += a;
-                sx[e] += a * xh;
-            }
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        red[0][threadIdx.x * V + e] = sd[e];
-        red[1][threadIdx.x * V + e] = sx[e];
+                for (int e = 0; e < V; ++e) {
+                    sd[e] += a[e];
+                    sx[e] = fmaf(a[e], xm[e], sx[e]);
+                }
+            });
     }
     __syncthreads();
-    const int S = p.VS * V;
+    float* red = lds;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        red[threadIdx.x * V + e] = sd[e];
+        red[(GN_THREADS + threadIdx.x) * V + e] = sx[e];
+    }
+    __syncthreads();
     float* out = (float*)p.partial + (((long long)n * p.chunks + blockIdx.x) * 2) * p.C + blockIdx.y * S;
     for (int j = threadIdx.x; j < S && blockIdx.y * S + j < p.C; j += GN_THREADS) {
         float a = 0.f, b = 0.f;
         for (int i = 0; i < p.PL; ++i) {
-            a += red[0][i * S + j];
-            b += red[1][i * S + j];
+            a += red[i * S + j];
+            b += red[GN_THREADS * V + i * S + j];
         }
         out[j] = a;
-        out[p.C + j] = b;
+        out[p.C + j] = b * p.stats[(p.N + n) * p.groups + (blockIdx.y * S + j) / p.Cg];
     }
 }
 
@@ -342,58 +520,483 @@ __global__ void __launch_bounds__(256) gn_bwd_terms_kernel(const GnParams p) {
     }
 }
 
-// dgamma, dbeta: the images' sums, in their order.
+// dgamma, dbeta: the images' sums.  A workgroup has 32 of the 2 C columns (d sums, then d * xh sums) and eight rows at a time.
 __global__ void __launch_bounds__(256) gn_bwd_params_kernel(const GnParams p) {
-    const int i = blockIdx.x * 256 + threadIdx.x;  // [0, 2C): d sums, then d * xh sums
-    if (i >= 2 * p.C) return;
+    __shared__ double red[8][32];
+    const int col = threadIdx.x & 31, row = threadIdx.x >> 5, i = blockIdx.x * 32 + col;
     double a = 0.0;
-    for (int n = 0; n < p.N; ++n) a += (double)p.sums[(long long)n * 2 * p.C + i];
-    if (i < p.C)
-        p.dbeta[i] = (float)a;
-    else
-        p.dgamma[i - p.C] = (float)a;
+    if (i < 2 * p.C)
+#pragma unroll 8
+        for (int n = row; n < p.N; n += 8) a += (double)p.sums[(long long)n * 2 * p.C + i];
+    red[row][col] = a;
+    __syncthreads();
+    if (row == 0 && i < 2 * p.C) {
+        for (int k = 1; k < 8; ++k) a += red[k][col];
+        if (i < p.C)
+            p.dbeta[i] = (float)a;
+        else
+            p.dgamma[i - p.C] = (float)a;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ backward, output
+// dx = d * scale - (x - mean) * (r r B) - r A, four pixels at a time.
 template <typename E, int ACT>
-__global__ void __launch_bounds__(GN_THREADS) gn_bwd_apply_kernel(const GnParams p) {
+__global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_apply_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
+    __shared__ __attribute__((aligned(16))) float lds[4 * GN_THREADS * V];
     const GnLane l = gn_lane<E>(p);
-    const int n = p.N - 1 - blockIdx.z, chunk = p.chunks - 1 - blockIdx.x;
+    const int n = p.N - 1 - blockIdx.z, chunk = p.chunks - 1 - blockIdx.x, S = p.VS * V;
     const int first = chunk * p.chunk, last = min(first + p.chunk, p.HW);
+    const float* mine = lds + (l.c - blockIdx.y * S);
+    gn_stage(lds, p, n, blockIdx.y * S, S);
     if (!l.on || first + l.pl >= last) return;
-    float mean[V], is[V], gamma[V], beta[V], A[V], B[V];
+    const GnConst<V> k(mine, S);
+    float k0[V], k1[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int g = (l.c + e) / p.Cg;
-        mean[e] = p.stats[n * p.groups + g];
-        is[e] = p.stats[(p.N + n) * p.groups + g];
-        A[e] = p.terms[n * p.groups + g];
-        B[e] = p.terms[(p.N + n) * p.groups + g];
-        gamma[e] = p.gamma[l.c + e];
-        beta[e] = p.beta[l.c + e];
+        const float r = p.stats[(p.N + n) * p.groups + g];
+        k0[e] = -r * p.terms[n * p.groups + g];
+        k1[e] = -r * r * p.terms[(p.N + n) * p.groups + g];
     }
+    const float near = gn_near<V>(k.beta);
     const int cb = l.c * (int)sizeof(E);
-    const char* x = p.x.p + n * p.x.img + cb;
-    const char* dy = p.dy.p + n * p.dy.img + cb;
-    char* y = p.y.p + n * p.y.img + cb;
+    const char* x = p.x.p + n * p.x.img;
+    const char* dy = p.dy.p + n * p.dy.img;
+    char* y = p.y.p + n * p.y.img;
     const int count = (last - first - l.pl + p.PL - 1) / p.PL;
-    GnCursor c(first + l.pl, p.PL, p.W);
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-        float v[V], d[V];
-        GnVec<E>::unpack(*(const u32x4*)(x + c.at(p.x)), v);
-        GnVec<E>::unpack(*(const u32x4*)(dy + c.at(p.dy)), d);
+    gn_with_stream(p.stream, [&](auto st) {
+        constexpr int ST = decltype(st)::value;
+        GnCursor<2> c(first + l.pl, p.PL, p.W, cb, {&p.x, &p.dy});
+        GnCursor<1> cy(first + l.pl, p.PL, p.W, cb, {&p.y});
+        gn_in_fours(count, [&](auto u) {
+            constexpr int U = decltype(u)::value;
+            u32x4 vr[U], dr[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                vr[i] = gn_load<ST>(x, c.at[0]);
+                dr[i] = gn_load<ST>(dy, c.at[1]);
+                c.next();
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                float xm[V], a[V];
+                gn_grads<E, ACT>(vr[i], dr[i], k, near, lds, l.c - blockIdx.y * S, S, p.slope, xm, a);
+#pragma unroll
+                for (int e = 0; e < V; ++e) a[e] = fmaf(a[e], k.scale[e], fmaf(xm[e], k1[e], k0[e]));
+                gn_store<ST>(y, cy.at[0], GnVec<E>::pack(a));
+                cy.next();
+            }
+        });
+    });
+}
+
+// ------------------------------------------------------------------------------------------------ whole images
+// One workgroup holds all pixels of a slab of whole groups of one image in registers, so that x (and dy) are read once: VS
+// vectors of 16 bytes per pixel, 64 / VS pixels next to each other in a wave, NV vectors to a thread.  The statistics are then
+// the two sums of the definition (mean, then squares about it), fp32 in a thread and fp64 between threads.
+constexpr int GN_SLAB = 128;  // most channels of a slab (at most the threads of the smallest workgroup)
+constexpr int GN_WAVES = 16;
+
+struct GnSeat {
+    int slab, n;
+    int wave, waves, pl, c, cs, first, step, count;  // c: channel; cs: channel in the slab; pixels first + i * step, i < count
+    int full, most;  // every lane has steps i < full, no lane has i >= most; most is full or full + 1
+    bool on;
+};
+template <typename E>
+__device__ __forceinline__ GnSeat gn_seat(const GnParams& p) {
+    GnSeat s;
+    // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of neighbouring slabs, so that slabs that share a
+    // cache line are read through one L2 at about the same time
+    const int total = p.slabs * p.N, q = total >> 3, rest = total & 7, xcd = blockIdx.x & 7;
+    const int at = xcd * q + min(xcd, rest) + (blockIdx.x >> 3);
+    s.n = at / p.slabs;
+    s.slab = at - s.n * p.slabs;
+    const int lane = threadIdx.x & 63;
+    s.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    s.waves = blockDim.x >> 6;
+    s.step = s.waves * p.PL;
+    s.full = p.HW / s.step;
+    s.most = (p.HW + s.step - 1) / s.step;
+    s.pl = lane / p.VS;
+    s.cs = (lane - s.pl * p.VS) * GnVec<E>::N;
+    s.c = s.slab * p.VS * GnVec<E>::N + s.cs;
+    s.on = s.pl < p.PL && s.c < p.C;
+    s.first = s.wave * p.PL + s.pl;
+    s.count = s.on && s.first < p.HW ? (p.HW - s.first + s.step - 1) / s.step : 0;
+    return s;
+}
+// The thread's vectors of K tensors; where it has none a load repeats its first one (or pixel 0's), so that all of them are plain
+// loads inside the view, issued one after the other.
+template <int K>
+struct GnWalk {
+    GnCursor<K> c;
+    int at0[K];
+    __device__ __forceinline__ GnWalk(const GnParams& p, const GnSeat& s, int cb, const GnTensor* const (&t)[K])
+        : c(s.count ? s.first : 0, s.step, p.W, cb, t) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) at0[k] = c.at[k];
+    }
+    template <int ST>
+    __device__ __forceinline__ u32x4 load(int k, int i, const GnSeat& s, const char* base) const {
+        return gn_load<ST>(base, i < s.count ? c.at[k] : at0[k]);
+    }
+};
+// ... and zeros there
+template <int NV>
+__device__ __forceinline__ void gn_blank(u32x4 (&v)[NV], const GnSeat& s) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (i >= s.full && i >= s.count) v[i] = u32x4{0u, 0u, 0u, 0u};
+}
+
+template <typename E>
+__device__ __forceinline__ void gn_put_four(u32x4& r, int h, const float* v) {
+    if constexpr (sizeof(E) == 2) {
+        r[2 * h] = pack_bf16x2(v[0], v[1]);
+        r[2 * h + 1] = pack_bf16x2(v[2], v[3]);
+    } else {
+        r = GnVec<float>::pack(v);
+    }
+}
+
+// A cursor over the thread's pixels whose positions the compiler does not keep from an earlier walk.
+template <int K>
+__device__ __forceinline__ GnCursor<K> gn_again(const GnParams& p, const GnSeat& s, int cb, const GnTensor* const (&t)[K]) {
+    int first = s.first;
+    asm volatile("" : "+v"(first));
+    return GnCursor<K>(first, s.step, p.W, cb, t);
+}
+
+// The sum over a wave's pixel lanes, valid in those of pixel lane 0.
+__device__ __forceinline__ float gn_over_pixels(float v, const GnParams& p, int pl, int top) {
+    for (int o = top; o; o >>= 1) {
+        const float w = __shfl_down(v, o * p.VS);
+        v += pl + o < p.PL ? w : 0.f;
+    }
+    return v;
+}
+
+// part[wave][cell] <- sums of the slab's cells (fold channels each) over the wave's pixels; then the group sums, handed to
+// done(group in the slab, sum, lane) in 16 lanes each.
+template <int V, typename F>
+__device__ __forceinline__ void gn_group_sums(float (&s)[V], float (*part)[GN_SLAB], const GnParams& p, const GnSeat& t, int groups,
+                                              int top, F done) {
+    if (p.fold >= 2)
+#pragma unroll
+        for (int e = 0; e < V; e += 2) s[e] += s[e + 1];
+    if (p.fold >= 4)
+#pragma unroll
+        for (int e = 0; e < V; e += 4) s[e] += s[e + 2];
+    if constexpr (V == 8)
+        if (p.fold >= 8) s[0] += s[4];
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if ((e & (p.fold - 1)) == 0) {
+            const float v = gn_over_pixels(s[e], p, t.pl, top);
+            if (t.pl == 0 && t.on) part[t.wave][(t.cs + e) / p.fold] = v;
+        }
+    __syncthreads();
+    const int cells = p.Cg / p.fold, items = cells * t.waves, sub = threadIdx.x & 15;  // 16 lanes to a group
+    for (int g0 = 0; g0 < groups; g0 += blockDim.x >> 4) {
+        const int g = g0 + (threadIdx.x >> 4);
+        double a = 0.0;
+        if (g < groups)
+            for (int i = sub; i < items; i += 16) {
+                const int w = i / cells;
+                a += (double)part[w][g * cells + i - w * cells];
+            }
+        for (int o = 8; o; o >>= 1) a += __shfl_xor(a, o);
+        if (g < groups) done(g, a, sub);
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ int gn_top(int pl) {  // the first distance of a tree over pl lanes
+    int o = 1;
+    while (o < pl) o <<= 1;
+    return o >> 1;
+}
+
+template <typename E, int ACT, int NV>
+__global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
+    constexpr int V = GnVec<E>::N;
+    __shared__ float part[GN_WAVES][GN_SLAB];
+    __shared__ __attribute__((aligned(16))) float mean_of[GN_SLAB], scale_of[GN_SLAB], shift_of[GN_SLAB];  // by channel
+    __shared__ double off_of[GN_SLAB];  // by group: the mean minus its fp32 value
+    const GnSeat t = gn_seat<E>(p);
+    const int n = t.n, S = p.VS * V, c0 = t.slab * S, g0 = c0 / p.Cg, top = gn_top(p.PL), width = min(S, p.C - c0);
+    const int groups = width / p.Cg;
+    const int cb = (t.on ? t.c : 0) * (int)sizeof(E);
+    const int mine = min((int)threadIdx.x, width - 1);  // width <= GN_SLAB <= threads; these two loads come back first
+    const float gamma = p.gamma[c0 + mine], beta = p.beta[c0 + mine];
+    const char* x = p.x.p + n * p.x.img;
+    u32x4 v[NV];
+    gn_with_stream(p.stream, [&](auto st) {
+        GnWalk<1> walk(p, t, cb, {&p.x});
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            v[i] = walk.template load<decltype(st)::value>(0, i, t, x);
+            walk.c.next();
+        }
+    });
+    gn_blank<NV>(v, t);
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (i < t.most) {
+            float f[V];
+            GnVec<E>::unpack(v[i], f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += f[e];
+        }
+    gn_group_sums<V>(s, part, p, t, groups, top, [&](int g, double sum, int sub) {
+        const double mean = sum * p.inv_count;
+        for (int i = sub; i < p.Cg; i += 16) mean_of[g * p.Cg + i] = (float)mean;
+        if (sub == 0) {
+            off_of[g] = mean - (double)(float)mean;
+            p.stats[n * p.groups + g0 + g] = (float)mean;
+        }
+    });
+    gn_forget<NV>(v);
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {  // four channels at a time: the registers are full
+        if (h) gn_forget<NV>(v);
+        float mean[4], q[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mean[e] = mean_of[t.cs + 4 * h + e];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < t.full || i < t.count) {
+                float f[4];
+                gn_part<E, 4>(v[i], h, f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float d = f[e] - mean[e];
+                    q[e] = fmaf(d, d, q[e]);
+                }
+            }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * h + e] = q[e];
+    }
+    gn_group_sums<V>(s, part, p, t, groups, top, [&](int g, double sum, int sub) {
+        const double off = off_of[g], var = sum * p.inv_count - off * off;
+        const float r = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps));
+        for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) scale_of[i] = r;
+        if (sub == 0) p.stats[(p.N + n) * p.groups + g0 + g] = r;
+    });
+    // fp32: (x - mean) * scale + beta; bf16: x * scale + (beta - mean * scale), whose rounding of mean * scale is far below the
+    // output's
+    constexpr bool SHIFT = sizeof(E) == 2;
+    if ((int)threadIdx.x < width) {
+        const float scale = gamma * scale_of[threadIdx.x];
+        scale_of[threadIdx.x] = scale;
+        shift_of[threadIdx.x] = SHIFT ? fmaf(-mean_of[threadIdx.x], scale, beta) : beta;
+    }
+    __syncthreads();
+    if (!t.count) return;
+    gn_forget<NV>(v);
+    const char* res = p.r.p ? p.r.p + n * p.r.img : nullptr;
+    char* y = p.y.p + n * p.y.img;
+    float mean[V], scale[V], shift[V];
+    auto constants = [&](int cs) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float xh = (v[e] - mean[e]) * is[e];
-            const float a = gn_act_grad<ACT>(d[e], v[e], xh, mean[e], is[e], gamma[e], beta[e], p.slope);
-            // the products are rounded one by one: with a single value in the group the terms cancel exactly
-            v[e] = ((gamma[e] * a - A[e]) - xh * B[e]) * is[e];
+            if (!SHIFT) mean[e] = mean_of[cs + e];
+            scale[e] = scale_of[cs + e];
+            shift[e] = shift_of[cs + e];
         }
-        *(u32x4*)(y + c.at(p.y)) = GnVec<E>::pack(v);
-        c.next();
+    };
+    constants(t.cs);
+    gn_with_stream(p.stream, [&](auto st) {
+        constexpr int ST = decltype(st)::value;
+        auto put = [&](int i, const u32x4* r, unsigned to) {
+            if constexpr (NV > 16) {  // no registers to keep them: from LDS for each vector
+                int cs = t.cs;
+                asm volatile("" : "+v"(cs));
+                constants(cs);
+            }
+            float f[V];
+            GnVec<E>::unpack(v[i], f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = gn_act<ACT>(fmaf(SHIFT ? f[e] : f[e] - mean[e], scale[e], shift[e]), p.slope);
+            if (r) {
+                float a[V];
+                GnVec<E>::unpack(*r, a);
+#pragma unroll
+                for (int e = 0; e < V; ++e) f[e] += a[e];
+            }
+            gn_store<ST>(y, to, GnVec<E>::pack(f));
+        };
+        if (res) {  // the residual of the next vectors is on its way while the last ones are finished
+            constexpr int AHEAD = NV > 16 ? 2 : 4;
+            GnWalk<1> ahead(p, t, cb, {&p.r});
+            GnCursor<1> c = gn_again<1>(p, t, cb, {&p.y});
+            u32x4 r[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD && i < NV; ++i) {
+                r[i] = ahead.template load<ST>(0, i, t, res);
+                ahead.c.next();
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const u32x4 now = r[i % AHEAD];
+                if (i + AHEAD < NV) {
+                    r[i % AHEAD] = ahead.template load<ST>(0, i + AHEAD, t, res);
+                    ahead.c.next();
+                }
+                if (i < t.count) put(i, &now, c.at[0]);
+                c.next();
+            }
+        } else {
+            GnCursor<1> c = gn_again<1>(p, t, cb, {&p.y});
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (i < t.count) put(i, nullptr, c.at[0]);
+                c.next();
+            }
+        }
+    });
+}
+
+// The backward pass the same way: x and dy in registers, the slab's sums per channel (they are also the image's share of dgamma
+// and dbeta), the group's two terms, dx.  Four channels at a time, so that the constants of a channel stay few.  In this form
+//   t = (x - mean) * (gamma r) + beta,   dx = d * (gamma r) - (x - mean) * (r r B) - r A.
+template <typename E, int ACT, int NV>
+__global__ void __launch_bounds__(1024) gn_whole_bwd_kernel(const GnParams p) {
+    constexpr int V = GnVec<E>::N, HALVES = V / 4;
+    enum { MEAN, R, GAMMA, BETA, C0, C1, KINDS };
+    __shared__ float part[2][GN_WAVES][GN_SLAB];
+    __shared__ float chan[2][GN_SLAB];
+    __shared__ __attribute__((aligned(16))) float of[KINDS][GN_SLAB];  // by channel
+    const GnSeat t = gn_seat<E>(p);
+    const int n = t.n, S = p.VS * V, c0 = t.slab * S, top = gn_top(p.PL), width = min(S, p.C - c0);
+    const int groups = width / p.Cg;
+    const int cb = (t.on ? t.c : 0) * (int)sizeof(E);
+    {   // these loads come back first
+        const int mine = min((int)threadIdx.x, width - 1), g = (c0 + mine) / p.Cg;
+        const float mean = p.stats[n * p.groups + g], r = p.stats[(p.N + n) * p.groups + g];
+        const float gamma = p.gamma[c0 + mine], beta = p.beta[c0 + mine];
+        if ((int)threadIdx.x < width) {
+            of[MEAN][mine] = mean;
+            of[R][mine] = r;
+            of[GAMMA][mine] = gamma;
+            of[BETA][mine] = beta;
+        }
     }
+    const char* xp = p.x.p + n * p.x.img;
+    const char* dp = p.dy.p + n * p.dy.img;
+    u32x4 x[NV], d[NV];
+    gn_with_stream(p.stream, [&](auto st) {
+        GnWalk<2> walk(p, t, cb, {&p.x, &p.dy});
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {  // in turn: the first pairs are used while the last ones are on their way
+            x[i] = walk.template load<decltype(st)::value>(0, i, t, xp);
+            d[i] = walk.template load<decltype(st)::value>(1, i, t, dp);
+            walk.c.next();
+        }
+    });
+    gn_blank<NV>(d, t);
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+        if (h) {
+            gn_forget<NV>(x);
+            gn_forget<NV>(d);
+        }
+        const int cs = t.cs + 4 * h;
+        const GnConst<4> k(&of[0][0] + cs, GN_SLAB);
+        const float near = gn_near<4>(k.beta);
+        float sd[4] = {0.f, 0.f, 0.f, 0.f}, sx[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < t.most) {  // where the thread has no pixel dy is zero
+                float xm[4], a[4];
+                gn_grads_of<E, ACT, 4>(x[i], d[i], h, k, near, &of[0][0], cs, GN_SLAB, p.slope, xm, a);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sd[e] += a[e];
+                    sx[e] = fmaf(a[e], xm[e], sx[e]);
+                }
+            }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float a = gn_over_pixels(sd[e], p, t.pl, top), b = gn_over_pixels(sx[e], p, t.pl, top);
+            if (t.pl == 0 && t.on) {
+                part[0][t.wave][t.cs + 4 * h + e] = a;
+                part[1][t.wave][t.cs + 4 * h + e] = b;
+            }
+        }
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < 2 * width; j += blockDim.x) {
+        const int which = j >= width, c = j - which * width;
+        float a = 0.f;
+        for (int w = 0; w < t.waves; ++w) a += part[which][w][c];
+        if (which) a *= of[R][c];
+        chan[which][c] = a;
+        p.sums[((long long)n * 2 + which) * p.C + c0 + c] = a;
+    }
+    __syncthreads();
+    const int sub = threadIdx.x & 15;
+    for (int h0 = 0; h0 < groups; h0 += blockDim.x >> 4) {
+        const int g = h0 + (threadIdx.x >> 4);
+        double A = 0.0, B = 0.0;
+        if (g < groups)
+            for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) {
+                const double gamma = of[GAMMA][i];
+                A += gamma * (double)chan[0][i];
+                B += gamma * (double)chan[1][i];
+            }
+        for (int o = 8; o; o >>= 1) {
+            A += __shfl_xor(A, o);
+            B += __shfl_xor(B, o);
+        }
+        if (g < groups)
+            for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) {
+                const double r = of[R][i];
+                of[C0][i] = (float)(-r * (A * p.inv_count));
+                of[C1][i] = (float)(-r * r * (B * p.inv_count));
+            }
+    }
+    __syncthreads();
+    if (!t.count) return;
+    char* y = p.y.p + n * p.y.img;
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) {
+        gn_forget<NV>(x);
+        gn_forget<NV>(d);
+        const int cs = t.cs + 4 * h;
+        const GnConst<4> k(&of[0][0] + cs, GN_SLAB);
+        const float near = gn_near<4>(k.beta);
+        float k0[4], k1[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            k0[e] = of[C0][cs + e];
+            k1[e] = of[C1][cs + e];
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < t.most) {
+                float xm[4], a[4];
+                gn_grads_of<E, ACT, 4>(x[i], d[i], h, k, near, &of[0][0], cs, GN_SLAB, p.slope, xm, a);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] = fmaf(a[e], k.scale[e], fmaf(xm[e], k1[e], k0[e]));
+                gn_put_four<E>(x[i], h, a);
+            }
+    }
+    gn_with_stream(p.stream, [&](auto st) {
+        GnCursor<1> c = gn_again<1>(p, t, cb, {&p.y});
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (i < t.count) gn_store<decltype(st)::value>(y, c.at[0], x[i]);
+            c.next();
+        }
+    });
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -440,9 +1043,53 @@ static void gn_split(GnParams& p, int es) {
     p.chunks = (int)((p.HW + chunk - 1) / chunk);
 }
 
+// Whether (and how) workgroups can hold the slabs of an image.  The slab's width, in bytes of a pixel, decides how whole the cache
+// lines are that a workgroup reads, its height in registers what fits; measured (bf16, 32 groups, time of one call in us):
+//   256 B where that leaves 512 workgroups       64 x 13 x 13 x 1024 backward 21.4, with 128 B 22.5
+//   128 B otherwise                              64 x 52 x 52 x 256 forward 36, with 64 B 49, in chunks 55
+//   narrower (to 32 B) for 256 workgroups        16 x 52 x 52 x 256 forward 16.2 with 32 B, 17.5 with 64 B, 24 with 128 B
+//   64 B so that it fits, no less                64 x 104 x 104 x 128 forward 102 with 32 B, in chunks 97
+// Forward a thread takes up to 11 vectors before the workgroup gets more waves (64 x 26 x 26 x 512: 17.8 us with 8 waves of 11, 23.3
+// with 16 of 6); backward it has two tensors' vectors, and spills above 8.
+struct GnWhole {
+    int VS, waves, NV;
+};
+static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out) {
+    const int V = 16 / es, vecs = p.C / V;
+    int unit = p.Cg;  // smallest slab: whole groups, whole vectors
+    while (unit % V) unit += p.Cg;
+    const int uv = unit / V, most = GN_SLAB / V < vecs ? GN_SLAB / V : vecs;
+    if (uv > most) return false;
+    const int nv_many = backward ? 6 : 11, nv_most = backward ? 8 : 22;
+    auto fit = [&](int vs) { return vs < uv ? uv : (vs < most ? vs : most) / uv * uv; };  // whole units, about vs vectors
+    auto blocks = [&](int vs) { return (long long)p.N * ((vecs + vs - 1) / vs); };
+    auto nv = [&](int vs, int waves) { return (p.HW + waves * (64 / vs) - 1) / (waves * (64 / vs)); };
+    int VS = fit(16);
+    if (blocks(VS) < 512 || nv(VS, GN_WAVES) > nv_most) VS = fit(8);
+    if (nv(VS, GN_WAVES) > nv_most) VS = fit(4);
+    if (blocks(VS) < 256 && VS > 4) VS = fit(4);
+    if (blocks(VS) < 256 && VS > 2) VS = fit(2);
+    int waves = 4;
+    while (waves < GN_WAVES && nv(VS, waves) > nv_many) waves *= 2;
+    out->VS = VS;
+    out->waves = waves;
+    out->NV = nv(VS, waves);
+    return out->NV <= nv_most;
+}
+
 static dim3 gn_grid(const GnParams& p, int es) {
     const int vecs = p.C * es / 16;
     return dim3(p.chunks, (vecs + p.VS - 1) / p.VS, p.N);
+}
+
+// A call that moves more than this leaves little of use in the 256 MB cache in front of HBM; its loads and stores go past the caches,
+// and what the first pass over x has left there stays for the second.  Measured (bf16, us): 64 x 208 x 208 x 64 forward 230 -> 193,
+// backward 347 -> 306; 64 x 52 x 52 x 256 forward 47 -> 36; 64 x 13 x 13 x 1024 backward (66 MB) 23.0 -> 21.8; below that it loses
+// (16 x 104 x 104 x 64 forward: 31.9 -> 33.4 us).  Only where a workgroup's stores are whole cache lines: narrower slabs share
+// them, and lose a factor of two and more.
+constexpr long long GN_STREAM_BYTES = 64ll << 20;
+static int gn_stream_rule(const GnParams& p, int es, int tensors) {
+    return (long long)tensors * p.N * p.HW * p.C * es >= GN_STREAM_BYTES;
 }
 
 static void gn_shape(GnParams& p, const yolo_view* x, int N, int C, int groups, int es) {
@@ -472,6 +1119,25 @@ using namespace yolo;
         else                                                                                                            \
             hipLaunchKernelGGL((KERNEL<float, GN_SILU>), grid, dim3(GN_THREADS), 0, st, p);                             \
     } while (0)
+
+#define GN_WHOLE_CASE(KERNEL, K)                                                                                           \
+    if (w.NV <= K) {                                                                                                       \
+        if (dtype == YOLO_BF16 && act == YOLO_ACT_LEAKY)                                                                   \
+            hipLaunchKernelGGL((KERNEL<unsigned short, GN_LEAKY, K>), grid, dim3(w.waves * 64), 0, st, p);                 \
+        else if (dtype == YOLO_BF16)                                                                                       \
+            hipLaunchKernelGGL((KERNEL<unsigned short, GN_SILU, K>), grid, dim3(w.waves * 64), 0, st, p);                  \
+        else if (act == YOLO_ACT_LEAKY)                                                                                    \
+            hipLaunchKernelGGL((KERNEL<float, GN_LEAKY, K>), grid, dim3(w.waves * 64), 0, st, p);                          \
+        else                                                                                                               \
+            hipLaunchKernelGGL((KERNEL<float, GN_SILU, K>), grid, dim3(w.waves * 64), 0, st, p);                           \
+    } else
+
+// The channels of a vector that always lie in one group: the largest power of two that divides both.
+static int gn_fold(int Cg, int V) {
+    int f = 1;
+    while (f < V && Cg % (2 * f) == 0) f *= 2;
+    return f;
+}
 
 extern "C" size_t yolo_gn_workspace_bytes(int N, int H, int W, int C, int groups, int dtype) {
     if (N <= 0 || H <= 0 || W <= 0 || C <= 0 || C % 8 || groups <= 0 || C % groups || (long long)H * W >= (1ll << 31)) return 0;
@@ -510,7 +1176,27 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
     p.partial = workspace;
     p.eps = eps;
     p.slope = leaky_slope;
+    p.stream = gn_stream_rule(p, es, residual ? 3 : 2);
     hipStream_t st = (hipStream_t)stream;
+    GnWhole w;
+    if (gn_whole_plan(p, es, false, &w)) {
+        p.VS = w.VS;
+        p.PL = 64 / w.VS;
+        p.fold = gn_fold(p.Cg, 16 / es);
+        p.slabs = (p.C * es / 16 + w.VS - 1) / w.VS;
+        p.stream = p.stream && w.VS % 8 == 0;  // whole cache lines only
+        const dim3 grid((unsigned)(p.slabs * N));
+        GN_WHOLE_CASE(gn_whole_kernel, 1)
+        GN_WHOLE_CASE(gn_whole_kernel, 2)
+        GN_WHOLE_CASE(gn_whole_kernel, 4)
+        GN_WHOLE_CASE(gn_whole_kernel, 6)
+        GN_WHOLE_CASE(gn_whole_kernel, 8)
+        GN_WHOLE_CASE(gn_whole_kernel, 11)
+        GN_WHOLE_CASE(gn_whole_kernel, 16)
+        GN_WHOLE_CASE(gn_whole_kernel, 22) { return fail(YOLO_E_ARG, "gn_act_fwd: no kernel for %d vectors", w.NV); }
+        YOLO_CHECK_HIP(hipGetLastError());
+        return YOLO_OK;
+    }
     const dim3 grid = gn_grid(p, es);
     if (dtype == YOLO_BF16)
         hipLaunchKernelGGL((gn_sums_kernel<unsigned short>), grid, dim3(GN_THREADS), 0, st, p);
@@ -550,12 +1236,30 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
     p.sums = (float*)workspace + (size_t)N * p.chunks * 2 * C;
     p.terms = p.sums + (size_t)N * 2 * C;
     p.slope = leaky_slope;
+    p.stream = gn_stream_rule(p, es, 3);
     hipStream_t st = (hipStream_t)stream;
+    const dim3 params_grid((2 * C + 31) / 32);
+    GnWhole w;
+    if (gn_whole_plan(p, es, true, &w)) {
+        p.VS = w.VS;
+        p.PL = 64 / w.VS;
+        p.slabs = (p.C * es / 16 + w.VS - 1) / w.VS;
+        p.stream = p.stream && w.VS % 8 == 0;  // whole cache lines only
+        const dim3 grid((unsigned)(p.slabs * N));
+        GN_WHOLE_CASE(gn_whole_bwd_kernel, 1)
+        GN_WHOLE_CASE(gn_whole_bwd_kernel, 2)
+        GN_WHOLE_CASE(gn_whole_bwd_kernel, 4)
+        GN_WHOLE_CASE(gn_whole_bwd_kernel, 6)
+        GN_WHOLE_CASE(gn_whole_bwd_kernel, 8) { return fail(YOLO_E_ARG, "gn_act_bwd: no kernel for %d vectors", w.NV); }
+        hipLaunchKernelGGL(gn_bwd_params_kernel, params_grid, dim3(256), 0, st, p);
+        YOLO_CHECK_HIP(hipGetLastError());
+        return YOLO_OK;
+    }
     const dim3 grid = gn_grid(p, es);
     GN_LAUNCH(gn_bwd_sums_kernel, grid, st, p);
     hipLaunchKernelGGL(gn_bwd_terms_kernel, dim3(groups, N), dim3(256), 0, st, p);
     GN_LAUNCH(gn_bwd_apply_kernel, grid, st, p);
-    hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((2 * C + 255) / 256), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(gn_bwd_params_kernel, params_grid, dim3(256), 0, st, p);
     YOLO_CHECK_HIP(hipGetLastError());
     return YOLO_OK;
 }
