@@ -444,29 +444,44 @@ def gn_workspace_bytes(N: int, H: int, W: int, C: int, groups: int, dtype: torch
     return int(lib().yolo_gn_workspace_bytes(N, H, W, C, groups, dtype_code(dtype)))
 
 
-def _check_gn(what: str, views, vectors, stats: torch.Tensor, workspace: torch.Tensor, groups: int, act: str) -> None:
-    first = views[0][1]
+def _gn_views(what: str, groups: int, act: str, views, vectors, stats: torch.Tensor, workspace: torch.Tensor):
+    """Checks of a group-norm call (single-image calls take a few microseconds on the GPU: these stay cheap); returns the
+    views' structs, the activation's code and the dtype's."""
+    (_, first), dt = views[0], views[0][1].buf.dtype
+    N, C = first.buf.shape[0], first.C
+    dev = first.buf.get_device()
+    if dev < 0 or dev != torch.cuda.current_device():
+        _require_cuda(first.buf, f"{what}: {views[0][0]}")
+    structs = []
     for name, v in views:
-        _require_cuda(v.buf, f"{what}: {name}")
+        buf = v.buf
+        if buf.get_device() != dev:
+            _require_cuda(buf, f"{what}: {name}")
         # the kernels address the view from its struct alone: the buffer behind it has to be what the struct says
-        if not v.buf.is_contiguous() or v.buf.dim() != 4 or v.buf.shape[1] != v.H + 2 * v.halo or v.buf.shape[2] != v.W + 2 * v.halo:
+        shape = buf.shape
+        if len(shape) != 4 or not buf.is_contiguous() or shape[1] != v.H + 2 * v.halo or shape[2] != v.W + 2 * v.halo:
             raise ValueError(f"{what}: {name}: a {v.H} x {v.W} view with halo {v.halo} does not describe its "
-                             f"{tuple(v.buf.shape)} buffer")
-        if v.buf.dtype != first.buf.dtype or (v.N, v.C) != (first.N, first.C):
-            raise ValueError(f"{what}: {name} is {v.N} x {v.C} channels of {v.buf.dtype}, expected {first.N} x {first.C} of "
-                             f"{first.buf.dtype}")
+                             f"{tuple(shape)} buffer")
+        if buf.dtype != dt or shape[0] != N or v.C != C:
+            raise ValueError(f"{what}: {name} is {shape[0]} x {v.C} channels of {buf.dtype}, expected {N} x {C} of {dt}")
+        structs.append(YoloView(buf.data_ptr(), v.H, v.W, v.halo, shape[3], v.ch_offset))
     for name, t in vectors:
-        _require_cuda(t, f"{what}: {name}")
-        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != first.C:
-            raise ValueError(f"{what}: {name} has to be a contiguous float32 vector of {first.C}")
-    _require_cuda(stats, f"{what}: stats")
-    if stats.dtype != torch.float32 or not stats.is_contiguous() or stats.numel() != 2 * first.N * groups:
-        raise ValueError(f"{what}: stats has to be a contiguous float32 tensor [2, {first.N}, {groups}]")
-    _require_cuda(workspace, f"{what}: workspace")
+        if t.get_device() != dev:
+            _require_cuda(t, f"{what}: {name}")
+        if t.dtype != torch.float32 or t.numel() != C or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} has to be a contiguous float32 vector of {C}")
+    if stats.get_device() != dev:
+        _require_cuda(stats, f"{what}: stats")
+    if stats.dtype != torch.float32 or stats.numel() != 2 * N * groups or not stats.is_contiguous():
+        raise ValueError(f"{what}: stats has to be a contiguous float32 tensor [2, {N}, {groups}]")
+    if workspace.get_device() != dev:
+        _require_cuda(workspace, f"{what}: workspace")
     if not workspace.is_contiguous():
         raise ValueError(f"{what}: workspace has to be contiguous")
-    if act not in ACTIVATIONS:
+    code = ACTIVATIONS.get(act)
+    if code is None:
         raise ValueError(f"{what}: activation {act!r} (one of {', '.join(ACTIVATIONS)})")
+    return structs, N, C, code, dtype_code(dt)
 
 
 def gn_act_fwd(x: View, gamma: torch.Tensor, beta: torch.Tensor, y: View, stats: torch.Tensor, workspace: torch.Tensor, *,
@@ -475,14 +490,11 @@ def gn_act_fwd(x: View, gamma: torch.Tensor, beta: torch.Tensor, y: View, stats:
     """y = act(group_norm(x) * gamma + beta) [+ residual]; stats [2, N, groups] f32 <- mean and 1 / sqrt(var + eps), for
     gn_act_bwd.  ``act``: "leaky" with ``slope`` in [0, 1] (1: no activation, 0: ReLU) or "silu".  ``y`` may be ``x`` or
     ``residual`` (each element is read before it is written); f32 or bf16, sums in f32 / f64."""
-    _check_gn("gn_act_fwd", [("x", x), ("y", y)] + ([("residual", residual)] if residual is not None else []),
-              [("gamma", gamma), ("beta", beta)], stats, workspace, groups, act)
-    xv, yv = x.c(), y.c()
-    rv = residual.c() if residual is not None else None
-    check(lib().yolo_gn_act_fwd(ctypes.byref(xv), _ptr(gamma), _ptr(beta), ctypes.byref(rv) if rv is not None else None,
-                                ctypes.byref(yv), _ptr(stats), x.N, x.C, groups, float(eps), ACTIVATIONS[act], float(slope),
-                                dtype_code(x.buf.dtype), _ptr(workspace), workspace.numel() * workspace.element_size(),
-                                _stream()), "yolo_gn_act_fwd")
+    views = (("x", x), ("y", y)) if residual is None else (("x", x), ("y", y), ("residual", residual))
+    v, N, C, code, dt = _gn_views("gn_act_fwd", groups, act, views, (("gamma", gamma), ("beta", beta)), stats, workspace)
+    check(lib().yolo_gn_act_fwd(v[0], gamma.data_ptr(), beta.data_ptr(), None if residual is None else v[2], v[1],
+                                stats.data_ptr(), N, C, groups, eps, code, slope, dt, workspace.data_ptr(),
+                                workspace.numel() * workspace.element_size(), _stream()), "yolo_gn_act_fwd")
 
 
 def gn_act_bwd(dy: View, x: View, gamma: torch.Tensor, beta: torch.Tensor, stats: torch.Tensor, dx: View,
@@ -490,13 +502,11 @@ def gn_act_bwd(dy: View, x: View, gamma: torch.Tensor, beta: torch.Tensor, stats
                slope: float = 0.1) -> None:
     """Backward of gn_act_fwd from its input and ``stats``: dx, dgamma [C], dbeta [C] (f32, overwritten).  The residual's
     gradient is dy itself.  ``dx`` may be ``dy`` or ``x``."""
-    _check_gn("gn_act_bwd", [("x", x), ("dy", dy), ("dx", dx)],
-              [("gamma", gamma), ("beta", beta), ("dgamma", dgamma), ("dbeta", dbeta)], stats, workspace, groups, act)
-    dyv, xv, dxv = dy.c(), x.c(), dx.c()
-    check(lib().yolo_gn_act_bwd(ctypes.byref(dyv), ctypes.byref(xv), _ptr(gamma), _ptr(beta), _ptr(stats), ctypes.byref(dxv),
-                                _ptr(dgamma), _ptr(dbeta), x.N, x.C, groups, ACTIVATIONS[act], float(slope),
-                                dtype_code(x.buf.dtype), _ptr(workspace), workspace.numel() * workspace.element_size(),
-                                _stream()), "yolo_gn_act_bwd")
+    v, N, C, code, dt = _gn_views("gn_act_bwd", groups, act, (("x", x), ("dy", dy), ("dx", dx)),
+                                  (("gamma", gamma), ("beta", beta), ("dgamma", dgamma), ("dbeta", dbeta)), stats, workspace)
+    check(lib().yolo_gn_act_bwd(v[1], v[0], gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), v[2], dgamma.data_ptr(),
+                                dbeta.data_ptr(), N, C, groups, code, slope, dt, workspace.data_ptr(),
+                                workspace.numel() * workspace.element_size(), _stream()), "yolo_gn_act_bwd")
 
 
 def wgrad_workspace_bytes(M: int, cin: int, cout: int, k: int) -> int:
@@ -995,10 +1005,11 @@ def grad_norm_workspace_bytes(table: GradTable) -> int:
     return int(lib().yolo_grad_norm_workspace_bytes(table.n_blocks))
 
 
-def _check_norms(t: Optional[torch.Tensor], n: int, what: str) -> None:
+def _check_norms(t: Optional[torch.Tensor], n: int, what: str, dev: int) -> None:
     if t is None:
         return
-    _require_cuda(t, what)
+    if t.get_device() != dev:
+        _require_cuda(t, what)
     if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n:
         raise ValueError(f"{what}: expected a contiguous float32 tensor of {n}")
 
@@ -1008,20 +1019,23 @@ def grad_norm(table: GradTable, norms: torch.Tensor, workspace: torch.Tensor, *,
     """norms [1] <- the norm (1, 2 or inf) of all the table's tensors together, or [n_tensors] <- of each; coefs, of the same
     length, <- min(1, max_norm / (norm + 1e-6)).  Nothing is read back to the host."""
     _require_cuda(table.blocks, "grad_norm")
-    n = table.n_tensors if per_tensor else 1
-    _check_norms(norms, n, "grad_norm: norms")
-    _check_norms(coefs, n, "grad_norm: coefs")
-    _require_cuda(workspace, "grad_norm: workspace")
-    check(lib().yolo_grad_norm(_ptr(table.blocks), table.n_blocks, _ptr(table.first) if per_tensor else None,
-                               table.n_tensors, float(norm_type), float(max_norm), _ptr(norms), _ptr(coefs), _ptr(workspace),
+    n, dev = table.n_tensors if per_tensor else 1, table.blocks.get_device()
+    _check_norms(norms, n, "grad_norm: norms", dev)
+    _check_norms(coefs, n, "grad_norm: coefs", dev)
+    if workspace.get_device() != dev:
+        _require_cuda(workspace, "grad_norm: workspace")
+    check(lib().yolo_grad_norm(table.blocks.data_ptr(), table.n_blocks, table.first.data_ptr() if per_tensor else None,
+                               table.n_tensors, norm_type, max_norm, norms.data_ptr(),
+                               None if coefs is None else coefs.data_ptr(), workspace.data_ptr(),
                                workspace.numel() * workspace.element_size(), _stream()), "yolo_grad_norm")
 
 
 def grad_scale(table: GradTable, coefs: torch.Tensor, *, per_tensor: bool = False) -> None:
     """Multiply the table's tensors by coefs [1], or each by its own of coefs [n_tensors], in place."""
     _require_cuda(table.blocks, "grad_scale")
-    _check_norms(coefs, table.n_tensors if per_tensor else 1, "grad_scale: coefs")
-    check(lib().yolo_grad_scale(_ptr(table.blocks), table.n_blocks, _ptr(coefs), int(per_tensor), _stream()), "yolo_grad_scale")
+    _check_norms(coefs, table.n_tensors if per_tensor else 1, "grad_scale: coefs", table.blocks.get_device())
+    check(lib().yolo_grad_scale(table.blocks.data_ptr(), table.n_blocks, coefs.data_ptr(), int(per_tensor), _stream()),
+          "yolo_grad_scale")
 
 
 def grad_clamp(table: GradTable, value: float) -> None:
@@ -1063,16 +1077,21 @@ def sgd_step_clipped(param: torch.Tensor, grad: torch.Tensor, mom: torch.Tensor,
                      per_tensor: bool = False, clip_value: Optional[float] = None) -> None:
     """sgd_step on clipped gradients, in the same one launch: grad times coefs [1] (or the factor of its tensor), or clamped to
     [-clip_value, clip_value].  ``grad`` itself is left as it is."""
+    _require_cuda(param, "sgd_step_clipped: param")
+    n, dev = param.numel(), param.get_device()
     for what, t in (("param", param), ("grad", grad), ("mom", mom)):
-        _require_cuda(t, f"sgd_step_clipped: {what}")
-        if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != param.numel():
-            raise ValueError(f"sgd_step_clipped: {what} has to be a contiguous float32 arena of {param.numel()} elements")
+        if t.get_device() != dev:
+            _require_cuda(t, f"sgd_step_clipped: {what}")
+        if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"sgd_step_clipped: {what} has to be a contiguous float32 arena of {n} elements")
     if (coefs is None) == (clip_value is None):
         raise ValueError("sgd_step_clipped: give coefs or clip_value, one of the two")
-    _require_cuda(table.blocks, "sgd_step_clipped: table")
-    if table.end > param.numel():
-        raise ValueError(f"sgd_step_clipped: the table covers {table.end} elements, the arenas have {param.numel()}")
-    _check_norms(coefs, table.n_tensors if per_tensor else 1, "sgd_step_clipped: coefs")
-    check(lib().yolo_sgd_step_clipped(_ptr(param), _ptr(grad), _ptr(mom), _ptr(table.blocks), table.n_blocks, lr0, wd0, lr1, wd1,
-                                      momentum, _ptr(coefs), int(per_tensor), -1.0 if clip_value is None else float(clip_value),
-                                      _stream()), "yolo_sgd_step_clipped")
+    if table.blocks.get_device() != dev:
+        _require_cuda(table.blocks, "sgd_step_clipped: table")
+    if table.end > n:
+        raise ValueError(f"sgd_step_clipped: the table covers {table.end} elements, the arenas have {n}")
+    _check_norms(coefs, table.n_tensors if per_tensor else 1, "sgd_step_clipped: coefs", dev)
+    check(lib().yolo_sgd_step_clipped(param.data_ptr(), grad.data_ptr(), mom.data_ptr(), table.blocks.data_ptr(),
+                                      table.n_blocks, lr0, wd0, lr1, wd1, momentum, None if coefs is None else coefs.data_ptr(),
+                                      int(per_tensor), -1.0 if clip_value is None else clip_value, _stream()),
+          "yolo_sgd_step_clipped")
