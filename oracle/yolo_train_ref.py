@@ -54,6 +54,9 @@ def conv_unit_train(x, sd, name: str, stride: int, pad: int, act: bool, frozen: 
     z = y
     if name + ".norm.weight" in sd:
         g, beta = sd[name + ".norm.weight"], sd[name + ".norm.bias"]
+        if name + ".norm.running_mean" not in sd:  # MODEL.DARKNET.NORM "GN": detectron2's GroupNorm(32, channels), frozen or not
+            y = F.group_norm(y, 32, g, beta, R.BN_EPS)
+            return F.leaky_relu(y, R.LEAKY) if act else y
         rm, rv = sd[name + ".norm.running_mean"], sd[name + ".norm.running_var"]
         if frozen:
             y = F.batch_norm(y, rm, rv, g, beta, False, BN_MOMENTUM, R.BN_EPS)

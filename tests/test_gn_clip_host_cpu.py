@@ -114,3 +114,40 @@ def test_clip_settings():
         with pytest.raises(ValueError):
             solver.build_optimizer(c, model)
     assert float(solver.clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0)) == 0.0
+
+
+def test_group_norm_network_is_built_and_refuses_what_it_cannot(tmp_path):
+    import workload
+    from yolo_amd.checkpoint import YOLOV3Checkpointer
+    from yolo_amd.checkpoint.load_darknet import save_darknet_weights
+    from yolo_amd.modeling.backbone.layers import GroupNorm, get_norm
+    from yolo_amd.utils.calibrate import calibrate_norm_stats
+    model, cfg = workload.build_model(config="yolov3.yaml", device="cpu", opts=["MODEL.DARKNET.NORM", "GN"])
+    convs = dict(model.backbone.darknet_modules())
+    norms = [c.norm for c in convs.values() if c.norm is not None]
+    assert len(norms) == 72 and all(isinstance(n, GroupNorm) and n.num_groups == 32 for n in norms)
+    keys = [k for k in model.state_dict() if ".norm." in k]
+    assert len(keys) == 144 and all(k.endswith((".norm.weight", ".norm.bias")) for k in keys)
+    w, b = convs["bottom_up.res2.0.conv1"].folded()
+    assert torch.equal(w, convs["bottom_up.res2.0.conv1"].weight) and float(b.abs().max()) == 0.0
+    opt = solver.build_optimizer(cfg, model)
+    assert sum(len(g["params"]) for g in opt.param_groups) == 210 and opt.param_groups[1]["weight_decay"] == 0.0
+    bn, _ = workload.build_model(config="yolov3.yaml", device="cpu")
+    path = str(tmp_path / "x.weights")
+    with open(path, "wb") as f:
+        save_darknet_weights(f, bn.backbone.darknet_modules())
+    with pytest.raises(ValueError, match="BatchNorm parameters"):
+        YOLOV3Checkpointer(model).load(path)
+    with open(path, "wb") as f, pytest.raises(ValueError, match="BatchNorm parameters"):
+        save_darknet_weights(f, model.backbone.darknet_modules())
+    with pytest.raises(ValueError, match="no running statistics"):
+        calibrate_norm_stats(model.backbone, torch.zeros(1, 3, 32, 32))
+    with pytest.raises(ValueError, match="do not divide"):
+        get_norm("GN", 48)
+    with pytest.raises(ValueError, match="not supported"):
+        get_norm("LN", 64)
+    # a checkpoint of the same network round-trips
+    torch.save({"model": model.state_dict()}, str(tmp_path / "gn.pth"))
+    other, _ = workload.build_model(config="yolov3.yaml", device="cpu", seed=1, opts=["MODEL.DARKNET.NORM", "GN"])
+    YOLOV3Checkpointer(other).load(str(tmp_path / "gn.pth"))
+    assert all(torch.equal(a, b) for a, b in zip(model.state_dict().values(), other.state_dict().values()))

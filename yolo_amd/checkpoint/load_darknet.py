@@ -24,6 +24,12 @@ def _take(buf: np.ndarray, pos: int, like: torch.Tensor) -> Tuple[torch.Tensor, 
     return torch.from_numpy(buf[pos:pos + n].copy()).view_as(like), pos + n
 
 
+def _needs_batch_norm(field: str, m) -> None:
+    if not hasattr(m.norm, "running_mean"):
+        raise ValueError(f"Darknet .weights files hold BatchNorm parameters and statistics; {field} of this model has a "
+                         f"{type(m.norm).__name__}")
+
+
 def load_darknet_weights_to_dict(f, module_list: Iterable, module_prefix: str = "backbone") -> Dict[str, torch.Tensor]:
     """f: binary file object; module_list: (name, conv) pairs in Darknet order (DarkNetFPN.darknet_modules())."""
     assert isinstance(f, io.IOBase)
@@ -36,6 +42,7 @@ def load_darknet_weights_to_dict(f, module_list: Iterable, module_prefix: str = 
     for field, m in module_list:
         name = f"{module_prefix}.{field}" if module_prefix else field
         if m.norm is not None:
+            _needs_batch_norm(field, m)
             for key, t in (("norm.bias", m.norm.bias), ("norm.weight", m.norm.weight),
                            ("norm.running_mean", m.norm.running_mean), ("norm.running_var", m.norm.running_var)):
                 sd[f"{name}.{key}"], pos = _take(buf, pos, t)
@@ -54,8 +61,9 @@ def load_darknet_weights_to_dict(f, module_list: Iterable, module_prefix: str = 
 def save_darknet_weights(f, module_list: Iterable, version=(0, 2, 5), seen: int = 0) -> None:
     """Inverse of the reader (used to produce fixtures and to export)."""
     np.array([version[0], version[1], version[2], seen & 0xFFFFFFFF, seen >> 32], dtype=np.int32).tofile(f)
-    for _, m in module_list:
+    for field, m in module_list:
         if m.norm is not None:
+            _needs_batch_norm(field, m)
             for t in (m.norm.bias, m.norm.weight, m.norm.running_mean, m.norm.running_var):
                 t.detach().cpu().float().numpy().tofile(f)
         else:

@@ -6,6 +6,8 @@ What is fused away relative to the reference's eager graph (all citations: refer
     (yolo/modeling/backbone/darknet.py:58-59,115-123; fpn.py:34-35,68-69,97-98);
   * ``residual = x.clone(); ...; out += residual`` (darknet.py:118,125): the conv2 launch adds the block
     input in its epilogue and writes IN PLACE over it (each element is read and written by one lane);
+    (GroupNorm -- MODEL.DARKNET.NORM "GN" -- cannot be folded: such a layer's convolution writes its raw output where the
+    activation belongs and the norm, activation and residual follow in place; the fused first stage is not used.)
   * ``nn.Upsample`` + ``torch.cat`` (fpn.py:36,179): the upsample conv writes each pixel 4x into channels
     [0, C/2) of the concat buffer, and the last block of res3/res4 writes its output straight into
     channels [C/2, ...) of the same buffer;
@@ -34,6 +36,7 @@ class PackedConv:
     cout: int
     k: int
     stride: int
+    gn: Optional[torch.nn.Module] = None   # the layer's GroupNorm (not folded)
 
 
 @dataclass
@@ -44,6 +47,7 @@ class Plan:
     steps: List[Callable[[], None]] = field(default_factory=list)
     stem_out: Optional[View] = None   # None when the stem is fused into the first down-sampling conv
     stem_fused_y: Optional[View] = None  # output of the fused stem + res1.downsample launch
+    stem_gn: Optional[tuple] = None   # (statistics, workspace) accessors of the stem's GroupNorm
     pre_steps: List[Callable[[], None]] = field(default_factory=list)  # fused launches that run before `steps`
     heads: List[View] = field(default_factory=list)  # p3, p4, p5
     taps: Dict[str, View] = field(default_factory=dict)
@@ -51,6 +55,7 @@ class Plan:
     decode_ws: Optional[torch.Tensor] = None
     nms_ws: Optional[torch.Tensor] = None
     splitk_ws: Dict[str, torch.Tensor] = field(default_factory=dict)  # partial-sum slabs of split-K layers, per stream
+    gn_bufs: Dict[tuple, object] = field(default_factory=dict)  # GroupNorm statistics, workspaces and scratch, per stream
     keep: Optional[torch.Tensor] = None
     n_keep: Optional[torch.Tensor] = None
     cand_cap: int = 0  # capacity wanted for the candidate buffers (0: the default of 4096 per image)
@@ -135,7 +140,8 @@ class Yolov3Engine:
                 pw, pb = ops.pack_stem(w, b, self.device)
             else:
                 pw, pb = ops.pack_conv(w, b, self.dtype, self.device)
-            self._packed[name] = PackedConv(pw, pb, conv.in_channels, conv.out_channels, conv.kernel_size, conv.stride)
+            self._packed[name] = PackedConv(pw, pb, conv.in_channels, conv.out_channels, conv.kernel_size, conv.stride,
+                                            conv.group_norm)
         self._plans.clear()
         self._graphs.clear()   # captured launches point at the old packed weights
 
@@ -156,6 +162,8 @@ class Yolov3Engine:
             c = pk[name]
             P.flops += 2 * N * (y.H // (2 if up else 1)) * (y.W // (2 if up else 1)) * c.cout * c.cin * c.k * c.k
             P.meta.append(dict(name=name, x=x, y=y, slope=slope, residual=residual, up=up))
+            if c.gn is not None:
+                return gn_conv(name, c, x, y, slope, residual, up)
             M = N * (y.H // (2 if up else 1)) * (y.W // (2 if up else 1))
             splits, nbytes = (ops.conv_splitk_plan(M, c.cin, c.cout, c.k, c.stride, dt)
                               if dt == torch.bfloat16 and self.split_k else (1, 0))
@@ -172,13 +180,43 @@ class Yolov3Engine:
             P.steps.append(lambda: ops.conv2d_fwd(x, c.w, c.b, y, cin=c.cin, cout=c.cout, k=c.k, stride=c.stride,
                                                   slope=slope, residual=residual, upsample2x=up))
 
+        def gn_conv(name: str, c: PackedConv, x: View, y: View, slope: float, residual: Optional[View], up: bool):
+            """A convolution with a GroupNorm behind it, one step: conv -> z (y itself, unless y holds the residual or is the
+            upsampled size), norm + activation + residual z -> y."""
+            key = "branch" if name.startswith(("fpn_output0.", "fpn_output1.")) else "main"   # as split-K's slabs
+            h, w = y.H // (2 if up else 1), y.W // (2 if up else 1)
+            z = y
+            if up or (residual is not None and residual.buf is y.buf):
+                zk = (key, h, w, c.cout)
+                if zk not in P.gn_bufs:
+                    P.gn_bufs[zk] = ops.alloc_view(N, h, w, c.cout, 0, dt, dev)
+                z = P.gn_bufs[zk]
+            stats, ws = self._gn_buffers(P, key, h, w, c.gn)
+            splits, nbytes = (ops.conv_splitk_plan(N * h * w, c.cin, c.cout, c.k, c.stride, dt)
+                              if dt == torch.bfloat16 and self.split_k else (1, 0))
+            if splits > 1 and (key not in P.splitk_ws or P.splitk_ws[key].numel() < nbytes):
+                P.splitk_ws[key] = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            kw = dict(cin=c.cin, cout=c.cout, k=c.k, stride=c.stride, slope=1.0)
+
+            def step():
+                if splits > 1:
+                    ops.conv2d_fwd_splitk(x, c.w, c.b, z, P.splitk_ws[key], **kw)
+                else:
+                    ops.conv2d_fwd(x, c.w, c.b, z, **kw)
+                c.gn.run(z, z if up else y, stats(), ws(), slope, residual)
+                if up:
+                    ops.upsample2x(z, y)
+            P.steps.append(step)
+
         stem = pk["bottom_up.stem.conv"]
         down0 = pk["bottom_up.res1.0.downsample"]
         # bf16: stem and the first stride-2 conv run as one launch, the stem output never reaches HBM
         fused = (self.fuse_stem and dt == torch.bfloat16 and stem.cout == 32 and down0.cout == 64
-                 and down0.k == 3 and down0.stride == 2)
+                 and down0.k == 3 and down0.stride == 2 and stem.gn is None and down0.gn is None)
         if not fused:
             P.stem_out = ops.alloc_view(N, H, W, stem.cout, 1, dt, dev)
+            if stem.gn is not None:
+                P.stem_gn = self._gn_buffers(P, "main", H, W, stem.gn)
         P.flops += 2 * N * H * W * stem.cout * 27
         x = P.stem_out
         h, w, c_in = H, W, stem.cout
@@ -250,6 +288,18 @@ class Yolov3Engine:
         P.taps.update(p3=heads[0], p4=heads[1], p5=heads[2])
         return P
 
+    def _gn_buffers(self, P: Plan, key: str, h: int, w: int, gn):
+        """Accessors of the (statistics, workspace) buffers that the GroupNorm layers of one stream of a plan share, grown to
+        what the largest of them needs while the plan is built."""
+        from .modeling.backbone.layers import gn_buffers
+        new = gn_buffers(P.N, h, w, gn, self.dtype, "meta")
+        G = gn.num_groups
+        need = {("stats", key, G): new[0], ("ws", key): new[1]}
+        for k, t in need.items():
+            if k not in P.gn_bufs or P.gn_bufs[k].numel() < t.numel():
+                P.gn_bufs[k] = torch.empty(t.shape, dtype=t.dtype, device=self.device)
+        return (lambda: P.gn_bufs[("stats", key, G)]), (lambda: P.gn_bufs[("ws", key)])
+
     # ------------------------------------------------------------------ execution
     @ops.on_own_device
     def run_backbone(self, images: torch.Tensor, mean=(0.0, 0.0, 0.0), std=(1.0, 1.0, 1.0),
@@ -296,7 +346,10 @@ class Yolov3Engine:
             ops.stem_down_fwd(images.contiguous(), stem.w, stem.b, d.w, d.b, P.stem_fused_y,
                               padded_hw=(P.H, P.W), mean=mean, std=std)
         else:
-            ops.stem_fwd(images.contiguous(), stem.w, stem.b, P.stem_out, mean=mean, std=std)
+            y = P.stem_out
+            ops.stem_fwd(images.contiguous(), stem.w, stem.b, y, mean=mean, std=std, slope=0.1 if stem.gn is None else 1.0)
+            if stem.gn is not None:
+                stem.gn.run(y, y, P.stem_gn[0](), P.stem_gn[1](), 0.1)
         for step in P.pre_steps:
             step()
 

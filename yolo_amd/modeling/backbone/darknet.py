@@ -10,7 +10,7 @@ import torch.nn as nn
 from ... import ops
 from ...structures import ShapeSpec
 from ..registry import BACKBONE_REGISTRY
-from .layers import Conv2d, c2_msra_fill, get_norm
+from .layers import Conv2d, c2_msra_fill, get_norm, gn_buffers
 
 LEAKY_SLOPE = 0.1  # darknet.py:59,116,120,123
 
@@ -58,7 +58,11 @@ class BasicStem(CNNBlockBase):
         N, _, H, W = x.shape
         w, b = self.conv.packed(dtype)
         y = ops.alloc_view(N, H, W, self.out_channels, 0, dtype, x.device)
-        ops.stem_fwd(x.float().contiguous(), w, b, y, mean=(0.0, 0.0, 0.0), std=(1.0, 1.0, 1.0), slope=LEAKY_SLOPE)
+        gn = self.conv.group_norm
+        ops.stem_fwd(x.float().contiguous(), w, b, y, mean=(0.0, 0.0, 0.0), std=(1.0, 1.0, 1.0),
+                     slope=LEAKY_SLOPE if gn is None else 1.0)
+        if gn is not None:
+            gn.run(y, y, *gn_buffers(N, H, W, gn, dtype, x.device), LEAKY_SLOPE)
         return y.nchw()
 
 

@@ -45,16 +45,48 @@ class BatchNorm2d(nn.Module):
         return dict(weight=self.weight, bias=self.bias, running_mean=self.running_mean, running_var=self.running_var)
 
 
+class GroupNorm(nn.Module):
+    """Group-norm parameters (detectron2's get_norm("GN") = torch.nn.GroupNorm(32, channels)).  Its statistics are each
+    image's own, so it is not folded into the convolution: it runs behind it, with the activation, as ops.gn_act_fwd."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5):
+        super().__init__()
+        if num_channels % num_groups:
+            raise ValueError(f"GroupNorm: {num_groups} groups do not divide {num_channels} channels")
+        self.num_groups, self.num_channels, self.eps = num_groups, num_channels, eps
+        self.weight = nn.Parameter(torch.ones(num_channels))
+        self.bias = nn.Parameter(torch.zeros(num_channels))
+
+    def as_dict(self):
+        return dict(weight=self.weight, bias=self.bias)
+
+    def run(self, z: ops.View, y: ops.View, stats: torch.Tensor, workspace: torch.Tensor, slope: float,
+            residual: Optional[ops.View] = None) -> None:
+        """y = leaky(norm(z)) [+ residual] on pixel-major views (y may be z)."""
+        ops.gn_act_fwd(z, self.weight.detach(), self.bias.detach(), y, stats, workspace, groups=self.num_groups, eps=self.eps,
+                       slope=slope, residual=residual)
+
+
+def gn_buffers(N: int, H: int, W: int, norm: GroupNorm, dtype: torch.dtype, device):
+    """(statistics, workspace) for GroupNorm.run on N x H x W pixels."""
+    C, G = norm.num_channels, norm.num_groups
+    return (torch.empty(2, N, G, device=device),
+            torch.empty(ops.gn_workspace_bytes(N, H, W, C, G, dtype), dtype=torch.uint8, device=device))
+
+
 def get_norm(norm: str, out_channels: int) -> Optional[nn.Module]:
     if norm in (None, ""):
         return None
     if norm in ("BN", "FrozenBN"):
         return BatchNorm2d(out_channels)
-    raise ValueError(f"norm '{norm}' is not supported on this path (the reference uses 'BN', defaults.py:19)")
+    if norm == "GN":
+        return GroupNorm(32, out_channels)
+    raise ValueError(f"norm '{norm}' is not supported on this path ('BN', the reference's, defaults.py:19; 'GN'; '')")
 
 
 class Conv2d(nn.Module):
-    """conv (+ folded norm) (+ LeakyReLU) (+ residual) as one HIP launch."""
+    """conv (+ folded norm) (+ LeakyReLU) (+ residual) as one HIP launch; with a GroupNorm the convolution alone, then the
+    norm, activation and residual."""
 
     def __init__(self, in_channels: int, out_channels: int, kernel_size: int, stride: int = 1, padding: int = 0,
                  bias: bool = True, norm: Optional[nn.Module] = None):
@@ -68,9 +100,17 @@ class Conv2d(nn.Module):
         nn.init.kaiming_uniform_(self.weight, a=5 ** 0.5)  # nn.Conv2d default (fpn.py:23-31 keeps it)
         self._packed = None  # (key, w_packed, bias_packed)
 
+    @property
+    def group_norm(self) -> Optional[GroupNorm]:
+        return self.norm if isinstance(self.norm, GroupNorm) else None
+
+    @property
+    def batch_norm(self) -> Optional[BatchNorm2d]:
+        return self.norm if isinstance(self.norm, BatchNorm2d) else None
+
     def folded(self):
-        return ops.fold_norm(self.weight, self.bias, self.norm.as_dict() if self.norm is not None else None,
-                             self.norm.eps if self.norm is not None else 1e-5)
+        bn = self.batch_norm
+        return ops.fold_norm(self.weight, self.bias, bn.as_dict() if bn is not None else None, bn.eps if bn is not None else 1e-5)
 
     def packed(self, dtype: torch.dtype):
         key = (dtype, self.weight._version, self.weight.device,
@@ -105,6 +145,11 @@ class Conv2d(nn.Module):
             raise RuntimeError("the 3-channel stem runs fused with pixel normalisation: call BasicStem")
         xv = ops.view_from_nchw(x, self.padding, dtype)
         rv = ops.view_from_nchw(residual, 0, dtype) if residual is not None else None
+        gn = self.group_norm
+        if gn is not None:
+            ops.conv2d_fwd(xv, w, b, y, cin=self.in_channels, cout=self.out_channels, k=k, stride=s, slope=1.0)
+            gn.run(y, y, *gn_buffers(N, Ho, Wo, gn, dtype, x.device), slope, rv)
+            return y.nchw()
         ops.conv2d_fwd(xv, w, b, y, cin=self.in_channels, cout=self.out_channels, k=k, stride=s, slope=slope,
                        residual=rv)
         return y.nchw()[:, :self.out_channels]

@@ -10,12 +10,13 @@ fpn.py:33-37,66-71,96-100,165-185 with the modules in training mode) is laid out
   backward, in reverse order:    yolo_bn_act_bwd(dy, z)                  ->  dz, dgamma, dbeta
                                  (its reduction pass comes out of the epilogue of the launch that wrote dy where
                                  that is the layer behind it: yolo_conv2d_fwd_bnbwd_sums + yolo_bn_act_bwd_presummed)
+                                 (a GroupNorm layer: yolo_gn_act_fwd / yolo_gn_act_bwd in the places of these)
                                  yolo_conv2d_wgrad(x, dz)                ->  dW
                                  yolo_conv2d_fwd(dz [dilated for stride 2], W^T rot180) (+ other consumers'
                                  gradient as the fused residual term)    ->  dx
 
 Frozen stages (cfg.MODEL.BACKBONE.FREEZE_AT, darknet.py:236-258: FrozenBatchNorm, no gradients) run as the
-fused inference kernels and take no part in the backward pass.  Activations are bf16 NHWC with a zero halo;
+fused inference kernels (with GroupNorm: convolution, then the norm in place) and take no part in the backward pass.  Activations are bf16 NHWC with a zero halo;
 every activation that backward needs has its own buffer (nothing is recomputed); weight, gamma and beta
 gradients are fp32.  nn.Upsample + torch.cat stay free in forward (channel slices of one buffer); their
 backward is a channel slice of the gradient buffer plus one 2x2-sum kernel.
@@ -86,7 +87,8 @@ class TPlan:
     norm: Optional[tuple] = None             # its (mean, std)
     stem_y: Optional[View] = None
     stem_out: Optional[View] = None
-    bn_ws: Optional[torch.Tensor] = None
+    bn_ws: Optional[torch.Tensor] = None     # workspace of the norms' launches, one after the other on the main stream
+    gn_stats: Dict[int, torch.Tensor] = field(default_factory=dict)  # frozen GroupNorm layers: statistics nobody reads again
     bn_sums: Optional[torch.Tensor] = None  # per-tile BatchNorm sums written by the conv epilogue
     wg_ws: Optional[torch.Tensor] = None
     arena: Optional[torch.Tensor] = None   # all parameter gradients, flat fp32, in backward order
@@ -259,7 +261,9 @@ class TrainEngine:
                 ho, wo = y.H, y.W
                 if conv.norm is not None:
                     L.z = A(ho, wo, conv.out_channels, 0)
-                    L.stats = torch.zeros(5, conv.out_channels, device=dev)
+                    gn = conv.group_norm
+                    L.stats = (torch.zeros(5, conv.out_channels, device=dev) if gn is None else
+                               torch.zeros(2, N, gn.num_groups, device=dev))
                     wide = A(ho, wo, (conv.out_channels + 63) // 64 * 64)   # zero-padded to what the data-gradient conv reads
                     L.dz = View(wide.buf, ho, wo, wide.halo, conv.out_channels, 0)
                 if conv.stride == 2 and not (dt == torch.bfloat16 and conv.kernel_size == 3 and conv.in_channels > 64):
@@ -284,7 +288,7 @@ class TrainEngine:
         cat = {3: A(H // 8, W // 8, chans[2] + chans[2] // 2), 4: A(H // 16, W // 16, chans[3] + chans[3] // 2)}
         h, w = H, W
         fused_prefix = (dt == torch.bfloat16 and stem.out_channels == 32 and c1 == 64 and self.blocks[0] >= 1
-                        and self.freeze_at >= 2)
+                        and self.freeze_at >= 2 and stem.group_norm is None)
         x = None
         stage_out: Dict[int, View] = {}
         if not fused_prefix:
@@ -382,6 +386,7 @@ class TrainEngine:
                     continue
                 Q, c = P.layers[i - 1], L.conv
                 if (c.stride == 1 and c.in_channels > 32 and c.in_channels % 8 == 0 and not Q.frozen and Q.z is not None
+                        and Q.conv.batch_norm is not None
                         and Q.up_dst is None and Q.y.buf is L.x.buf and Q.y.ch_offset == L.x.ch_offset
                         and Q.y.C == L.x.C == L.x.buf.shape[3] and min(writers[id(L.dx.buf)]) == i):
                     L.sums_for = Q
@@ -405,7 +410,9 @@ class TrainEngine:
             else:
                 L.dbias = P.arena[off:off + c.out_channels]
             L.arena_end = end
-        n_bn = max(ops.bn_workspace_bytes(N, L.y.H, L.y.W, L.conv.out_channels) for L in P.layers if L.z is not None)
+        n_bn = max([ops.bn_workspace_bytes(N, L.y.H, L.y.W, L.conv.out_channels) if L.conv.group_norm is None else
+                    self._gn_bytes(N, L.y, L.conv) for L in P.layers if L.z is not None or L.conv.group_norm is not None] +
+                   ([self._gn_bytes(N, P.stem_out, stem)] if stem.group_norm is not None else []))
         P.bn_ws = torch.empty(n_bn, dtype=torch.uint8, device=dev)
         n_sums = max([ops.conv_bnsums_rows(L.x, L.z, L.conv.in_channels, L.conv.out_channels, L.conv.kernel_size,
                                            L.conv.stride) * 2 * L.conv.out_channels
@@ -425,8 +432,19 @@ class TrainEngine:
         (32 output channels, or 32 input channels under a 3x3 bf16 filter: kernel instances without that epilogue) and
         the stem take the separate statistics pass."""
         c = L.conv
-        return (self.fuse_bn_sums and L.z is not None and not L.stem and c.out_channels > 32
+        return (self.fuse_bn_sums and L.z is not None and not L.stem and c.out_channels > 32 and c.batch_norm is not None
                 and not (self.dtype == torch.bfloat16 and c.in_channels == 32 and c.kernel_size == 3))
+
+    def _gn_bytes(self, N: int, y: View, conv) -> int:
+        return ops.gn_workspace_bytes(N, y.H, y.W, conv.out_channels, conv.group_norm.num_groups, self.dtype)
+
+    def _gn_in_place(self, P: TPlan, conv, y: View, slope: float, residual: Optional[View] = None) -> None:
+        """A frozen layer's GroupNorm over its convolution's output in ``y``; the statistics are not kept."""
+        gn = conv.group_norm
+        key = gn.num_groups
+        if key not in P.gn_stats:
+            P.gn_stats[key] = torch.empty(2, P.N, key, device=self.device)
+        gn.run(y, y, P.gn_stats[key], P.bn_ws, slope, residual)
 
     @staticmethod
     def _is_conv1(L: TLayer) -> bool:
@@ -437,6 +455,11 @@ class TrainEngine:
             if M.y.buf is L.x.buf and M is not L:
                 return M.frozen
         return True  # produced by the fused frozen prefix
+
+    @staticmethod
+    def _running(norm, update: bool):
+        """The running statistics a training-mode BatchNorm updates (none: a GroupNorm, or no update wanted)."""
+        return (norm.running_mean, norm.running_var) if update and hasattr(norm, "running_mean") else (None, None)
 
     # ------------------------------------------------------------------ forward
     @ops.on_own_device
@@ -457,19 +480,31 @@ class TrainEngine:
                 for step in P.prefix:
                     step()
             else:
-                ops.stem_fwd(images, stem_w, stem_b, P.stem_out, mean=mean, std=std)
+                conv = self.convs["bottom_up.stem.conv"]
+                ops.stem_fwd(images, stem_w, stem_b, P.stem_out, mean=mean, std=std,
+                             slope=LEAKY if conv.group_norm is None else 1.0)
+                if conv.group_norm is not None:
+                    self._gn_in_place(P, conv, P.stem_out, LEAKY)
         for L in P.layers:
             c = L.conv
             if L.stem:   # normalisation + 3 -> 32 convolution from the images, then batch statistics like any layer
                 n = c.norm
-                rm, rv = (n.running_mean, n.running_var) if update_running_stats else (None, None)
+                rm, rv = self._running(n, update_running_stats)
                 ops.stem_fwd(images, self._stem_w, self._zeros(c.out_channels), L.z, mean=mean, std=std, slope=1.0)
+                if c.group_norm is not None:
+                    n.run(L.z, L.y, L.stats, P.bn_ws, L.slope)
+                    continue
                 ops.bn_train_stats(L.z, n.weight.detach(), n.bias.detach(), L.stats, P.bn_ws, eps=n.eps,
                                    momentum=BN_MOMENTUM, running_mean=rm, running_var=rv)
                 ops.bn_act_fwd(L.z, L.stats, L.y, slope=L.slope)
                 continue
             if L.frozen:
                 w, b = self._packed(L.name, "folded")
+                if c.group_norm is not None:
+                    ops.conv2d_fwd(L.x, w, b, L.y, cin=c.in_channels, cout=c.out_channels, k=c.kernel_size,
+                                   stride=c.stride, slope=1.0)
+                    self._gn_in_place(P, c, L.y, L.slope, L.residual)
+                    continue
                 ops.conv2d_fwd(L.x, w, b, L.y, cin=c.in_channels, cout=c.out_channels, k=c.kernel_size, stride=c.stride,
                                slope=L.slope, residual=L.residual)
                 continue
@@ -479,7 +514,14 @@ class TrainEngine:
                                slope=1.0)
                 continue
             n = c.norm
-            rm, rv = (n.running_mean, n.running_var) if update_running_stats else (None, None)
+            if c.group_norm is not None:
+                ops.conv2d_fwd(L.x, w, b, L.z, cin=c.in_channels, cout=c.out_channels, k=c.kernel_size, stride=c.stride,
+                               slope=1.0)
+                n.run(L.z, L.y, L.stats, P.bn_ws, L.slope, L.residual)
+                if L.up_dst is not None:
+                    ops.upsample2x(L.y, L.up_dst)
+                continue
+            rm, rv = self._running(n, update_running_stats)
             if self._sums_in_epilogue(L):   # the conv epilogue leaves per-tile sums of z and z*z: no second pass over z
                 rows = ops.conv2d_fwd_bnsums(L.x, w, b, L.z, P.bn_sums, cin=c.in_channels, cout=c.out_channels,
                                              k=c.kernel_size, stride=c.stride)
@@ -529,7 +571,11 @@ class TrainEngine:
             else:
                 if L.up_src is not None:
                     ops.sum2x2(L.up_src, L.dy)
-                if L.presummed_rows:   # the launch that wrote dy (the previous step of this loop) left the reduction
+                gn = c.group_norm
+                if gn is not None:
+                    ops.gn_act_bwd(L.dy, L.z, gn.weight.detach(), gn.bias.detach(), L.stats, L.dz, L.dgamma, L.dbeta, P.bn_ws,
+                                   groups=gn.num_groups, slope=L.slope)
+                elif L.presummed_rows:   # the launch that wrote dy (the previous step of this loop) left the reduction
                     ops.bn_act_bwd_presummed(L.dy, L.z, L.stats, L.dz, L.dgamma, L.dbeta, P.bn_sums, L.presummed_rows,
                                              slope=L.slope)
                     L.presummed_rows = 0

@@ -29,6 +29,8 @@ def calibrate_norm_stats(backbone, images: torch.Tensor, mean=(0.0, 0.0, 0.0), s
     residual networks start from) gives a well-conditioned network, which is what a test needs when it wants to see
     the arithmetic error of the kernels rather than the network's own sensitivity."""
     from ..engine import Yolov3Engine
+    if any(conv.group_norm is not None for _, conv in backbone.darknet_modules()):
+        raise ValueError("calibrate_norm_stats: a GroupNorm has no running statistics to estimate")
     dev = next(backbone.parameters()).device
     if dev.type == "cuda" and dev.index != torch.cuda.current_device():  # launch on the GPU that holds the model
         with torch.cuda.device(dev):
