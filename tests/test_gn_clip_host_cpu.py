@@ -44,6 +44,10 @@ def test_gn_refusals_of_one_direction():
     assert "y is 8 x 9" in _fwd(y=_view(W=9))[1] and "residual is 7 x 8" in _fwd(r=_view(H=7))[1]
     assert "eps" in _fwd(eps=-1.0)[1] and "dy is 9 x 8" in _bwd(dy=_view(H=9))[1] and "dx is 8 x 4" in _bwd(dx=_view(W=4))[1]
     assert _fwd(ws=16)[0] == -2
+    wide = lambda at, halo=0: _view(halo=halo, total=192, at=at)  # noqa: E731
+    for kw in (dict(x=wide(0), y=wide(8)), dict(x=wide(64), y=wide(64, 1)), dict(x=wide(128), y=wide(0), r=wide(56))):
+        assert "lies over part" in _fwd(**kw)[1]
+    assert "lies over part of dy" in _bwd(x=wide(0), dx=wide(64), dy=wide(72))[1]
     L = _lib.lib()
     assert L.yolo_gn_workspace_bytes(0, 8, 8, 64, 32, 1) == 0 and L.yolo_gn_workspace_bytes(1, 8, 8, 60, 4, 1) == 0
     assert L.yolo_gn_workspace_bytes(64, 208, 208, 64, 32, 1) > 0

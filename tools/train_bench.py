@@ -25,6 +25,8 @@ def main():
     ap.add_argument("--size", type=int, default=416)
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
+    ap.add_argument("--opts", nargs=argparse.REMAINDER, default=[], help="config overrides, e.g. MODEL.DARKNET.NORM GN "
+                    "SOLVER.CLIP_GRADIENTS.ENABLED True SOLVER.CLIP_GRADIENTS.CLIP_TYPE full_model")
     args = ap.parse_args()
     if os.environ.get("YOLO_DEBUG_HANG"):   # dump every thread's stack and exit if the run takes this many seconds
         import faulthandler
@@ -32,7 +34,7 @@ def main():
     world, rank, local = D.init_from_env("nccl")
     torch.cuda.set_device(local if world > 1 else 0)
     model, cfg = workload.build_model(config=args.config, dtype="bf16", device=f"cuda:{torch.cuda.current_device()}",
-                                      opts=["OUTPUT_DIR", "", "SOLVER.CHECKPOINT_PERIOD", 0, "SOLVER.BASE_LR", 1e-4])
+                                      opts=["OUTPUT_DIR", "", "SOLVER.CHECKPOINT_PERIOD", 0, "SOLVER.BASE_LR", 1e-4] + args.opts)
     # one resident batch, reused: the loop measures the step, not the synthetic generator
     batch = next(synthetic_batches(cfg, args.batch, args.size, seed=7 + rank, device=model.device))
     tr = Trainer(cfg, model, iter(lambda: batch, None), log=lambda m: None)

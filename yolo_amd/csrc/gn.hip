@@ -11,6 +11,8 @@
 //
 // Memory-bound: a pass reads or writes 16 bytes per lane, sums are fp32 within a thread (about a pivot where squares would
 // cancel) and fp64 from there on.
+#include <type_traits>
+
 #include "common.h"
 
 namespace yolo {
@@ -42,7 +44,7 @@ struct GnParams {
 };
 
 constexpr int GN_THREADS = 256;
-constexpr int GN_MAX_CHUNKS = 64;
+constexpr int GN_MAX_CHUNKS = 256;
 
 template <typename E> struct GnVec;
 template <> struct GnVec<unsigned short> {
@@ -342,26 +344,64 @@ __global__ void __launch_bounds__(GN_THREADS, 5) gn_sums_kernel(const GnParams p
     }
 }
 
-// One workgroup per (group, image): chunk sums -> mean and r.
-__global__ void __launch_bounds__(64) gn_stats_kernel(const GnParams p) {
-    const int g = blockIdx.x, n = blockIdx.y, total = p.chunks * p.Cg;
-    const double* part = (const double*)p.partial + (long long)n * p.chunks * 2 * p.C + g * p.Cg;
-    double s = 0.0, q = 0.0;
-    for (int i = threadIdx.x; i < total; i += 64) {
-        const int ch = i / p.Cg, c = i - ch * p.Cg;
-        s += part[(long long)ch * 2 * p.C + c];
-        q += part[((long long)ch * 2 + 1) * p.C + c];
+// The chunks' sums of the groups of about 64 channels of one image, in fp64 and in the chunks' order: lanes are channels, the
+// sixteen waves take the chunks in turn.  Forward: mean and r of a group.  Backward: the image's sums of each channel, and the group's two
+// terms from gamma times them.
+constexpr int GN_JOIN = 16;
+template <bool BWD>
+__global__ void __launch_bounds__(GN_JOIN * 64) gn_join_kernel(const GnParams p) {
+    typedef typename std::conditional<BWD, float, double>::type P;
+    __shared__ double red[2][GN_JOIN][64];
+    const int col = threadIdx.x & 63, row = threadIdx.x >> 6, n = blockIdx.y;
+    const int per = p.Cg < 64 ? 64 / p.Cg : 1, g0 = blockIdx.x * per, groups = min(per, p.groups - g0), width = groups * p.Cg;
+    const P* part = (const P*)p.partial + (long long)n * p.chunks * 2 * p.C + g0 * p.Cg;
+    double A = 0.0, B = 0.0;
+    for (int c0 = 0; c0 < width; c0 += 64) {
+        const int c = c0 + col;
+        double a = 0.0, b = 0.0;
+        if (c < width)
+#pragma unroll 4
+            for (int i = row; i < p.chunks; i += GN_JOIN) {
+                a += (double)part[(long long)i * 2 * p.C + c];
+                b += (double)part[((long long)i * 2 + 1) * p.C + c];
+            }
+        red[0][row][col] = a;
+        red[1][row][col] = b;
+        __syncthreads();
+        if (row == 0) {
+            for (int w = 1; w < GN_JOIN; ++w) {
+                a += red[0][w][col];
+                b += red[1][w][col];
+            }
+            if (BWD && c < width) {
+                p.sums[((long long)n * 2) * p.C + g0 * p.Cg + c] = (float)a;
+                p.sums[((long long)n * 2 + 1) * p.C + g0 * p.Cg + c] = (float)b;
+                const double gamma = p.gamma[g0 * p.Cg + c];
+                a *= gamma;
+                b *= gamma;
+            }
+            red[0][0][col] = a;
+            red[1][0][col] = b;
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < groups) {  // groups > 1: all their channels are here; else the next 64 of the one group
+            const int first = groups > 1 ? threadIdx.x * p.Cg : 0, last = groups > 1 ? first + p.Cg : min(64, width - c0);
+            for (int i = first; i < last; ++i) {
+                A += red[0][0][i];
+                B += red[1][0][i];
+            }
+        }
+        __syncthreads();
     }
-    for (int o = 32; o; o >>= 1) {
-        s += __shfl_xor(s, o);
-        q += __shfl_xor(q, o);
-    }
-    if (threadIdx.x == 0) {
-        const double mean = s * p.inv_count;
-        double var = q * p.inv_count - mean * mean;
-        var = var < 0.0 ? 0.0 : var;
-        p.stats[n * p.groups + g] = (float)mean;
-        p.stats[(p.N + n) * p.groups + g] = (float)(1.0 / sqrt(var + (double)p.eps));
+    if ((int)threadIdx.x >= groups) return;
+    const int g = n * p.groups + g0 + threadIdx.x;
+    if (BWD) {
+        p.terms[g] = (float)(A * p.inv_count);
+        p.terms[p.N * p.groups + g] = (float)(B * p.inv_count);
+    } else {
+        const double mean = A * p.inv_count, var = B * p.inv_count - mean * mean;
+        p.stats[g] = (float)mean;
+        p.stats[p.N * p.groups + g] = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps));
     }
 }
 
@@ -479,44 +519,6 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_sums_kernel(const GnPara
         }
         out[j] = a;
         out[p.C + j] = b * p.stats[(p.N + n) * p.groups + (blockIdx.y * S + j) / p.Cg];
-    }
-}
-
-// One workgroup per (group, image): chunk sums -> the image's sums per channel and the group's two terms.
-__global__ void __launch_bounds__(256) gn_bwd_terms_kernel(const GnParams p) {
-    __shared__ double ra[4], rb[4];
-    const int g = blockIdx.x, n = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const float* part = (const float*)p.partial + (long long)n * p.chunks * 2 * p.C;
-    double A = 0.0, B = 0.0;
-    for (int j = wave; j < p.Cg; j += 4) {
-        const int c = g * p.Cg + j;
-        double a = 0.0, b = 0.0;
-        for (int i = lane; i < p.chunks; i += 64) {
-            a += (double)part[(long long)i * 2 * p.C + c];
-            b += (double)part[((long long)i * 2 + 1) * p.C + c];
-        }
-        for (int o = 32; o; o >>= 1) {
-            a += __shfl_xor(a, o);
-            b += __shfl_xor(b, o);
-        }
-        const double gamma = p.gamma[c];
-        A += gamma * a;
-        B += gamma * b;
-        if (lane == 0) {
-            p.sums[((long long)n * 2) * p.C + c] = (float)a;
-            p.sums[((long long)n * 2 + 1) * p.C + c] = (float)b;
-        }
-    }
-    if (lane == 0) {
-        ra[wave] = A;
-        rb[wave] = B;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        A = ra[0] + ra[1] + ra[2] + ra[3];
-        B = rb[0] + rb[1] + rb[2] + rb[3];
-        p.terms[n * p.groups + g] = (float)(A * p.inv_count);
-        p.terms[(p.N + n) * p.groups + g] = (float)(B * p.inv_count);
     }
 }
 
@@ -1012,6 +1014,15 @@ static int gn_check_view(const yolo_view* v, const yolo_view* like, int N, int C
     return YOLO_OK;
 }
 
+// An output over an input: all of it in place, or none of it.
+static int gn_check_overlap(const yolo_view* out, const yolo_view* in, int C, const char* op, const char* what) {
+    if (out->ptr != in->ptr || (out->ch_offset == in->ch_offset && out->ch_total == in->ch_total && out->halo == in->halo)) return YOLO_OK;
+    YOLO_REQUIRE(out->ch_total == in->ch_total && out->halo == in->halo &&
+                     (out->ch_offset + C <= in->ch_offset || in->ch_offset + C <= out->ch_offset),
+                 "%s: the output lies over part of %s", op, what);
+    return YOLO_OK;
+}
+
 static GnTensor gn_tensor(const yolo_view* v, int es) {
     const ViewGeom g = geom_of(*v);
     return GnTensor{(char*)v->ptr + (long long)g.origin * es, g.img_stride * es, g.row_stride * es, g.pix_stride * es};
@@ -1027,8 +1038,8 @@ static int gn_check_shape(int N, int C, int groups, int act, float slope, int dt
     return YOLO_OK;
 }
 
-// The split of an image over workgroups: pixel chunks so that about 2048 workgroups (8 per CU) are there, but no more than 64
-// chunks and no fewer than 4 pixels to a thread.
+// The split of an image over workgroups: pixel chunks so that about 2048 workgroups (8 per CU) are there, but no more than 256
+// chunks for that (what joins them reads them all), no fewer than 4 pixels to a thread, and no more than 128 (its fp32 sums).
 static void gn_split(GnParams& p, int es) {
     const int vecs = p.C * es / 16;
     p.VS = vecs < GN_THREADS ? vecs : GN_THREADS;
@@ -1039,6 +1050,7 @@ static void gn_split(GnParams& p, int es) {
     if (want > GN_MAX_CHUNKS) want = GN_MAX_CHUNKS;
     long long chunk = (p.HW + want - 1) / want;
     if (chunk < 4ll * p.PL) chunk = 4ll * p.PL;
+    if (chunk > 128ll * p.PL) chunk = 128ll * p.PL;
     p.chunk = (int)chunk;
     p.chunks = (int)((p.HW + chunk - 1) / chunk);
 }
@@ -1048,7 +1060,7 @@ static void gn_split(GnParams& p, int es) {
 //   256 B where that leaves 512 workgroups       64 x 13 x 13 x 1024 backward 21.4, with 128 B 22.5
 //   128 B otherwise                              64 x 52 x 52 x 256 forward 36, with 64 B 49, in chunks 55
 //   narrower (to 32 B) for 256 workgroups        16 x 52 x 52 x 256 forward 16.2 with 32 B, 17.5 with 64 B, 24 with 128 B
-//   64 B so that it fits, no less                64 x 104 x 104 x 128 forward 102 with 32 B, in chunks 97
+//   64 B so that it fits, no less                64 x 104 x 104 x 128 forward 102 with 32 B, in chunks 97; one image 33 and 18
 // Forward a thread takes up to 11 vectors before the workgroup gets more waves (64 x 26 x 26 x 512: 17.8 us with 8 waves of 11, 23.3
 // with 16 of 6); backward it has two tensors' vectors, and spills above 8.
 struct GnWhole {
@@ -1067,6 +1079,7 @@ static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out
     int VS = fit(16);
     if (blocks(VS) < 512 || nv(VS, GN_WAVES) > nv_most) VS = fit(8);
     if (nv(VS, GN_WAVES) > nv_most) VS = fit(4);
+    if (nv(VS, GN_WAVES) > nv_most) return false;
     if (blocks(VS) < 256 && VS > 4) VS = fit(4);
     if (blocks(VS) < 256 && VS > 2) VS = fit(2);
     int waves = 4;
@@ -1074,7 +1087,12 @@ static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out
     out->VS = VS;
     out->waves = waves;
     out->NV = nv(VS, waves);
-    return out->NV <= nv_most;
+    return true;
+}
+
+static dim3 gn_join_grid(const GnParams& p) {
+    const int per = p.Cg < 64 ? 64 / p.Cg : 1;
+    return dim3((p.groups + per - 1) / per, p.N);
 }
 
 static dim3 gn_grid(const GnParams& p, int es) {
@@ -1161,6 +1179,9 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
     if (int e = gn_check_view(y, x, N, C, es, "gn_act_fwd", "y")) return e;
     if (residual)
         if (int e = gn_check_view(residual, x, N, C, es, "gn_act_fwd", "residual")) return e;
+    if (int e = gn_check_overlap(y, x, C, "gn_act_fwd", "x")) return e;
+    if (residual)
+        if (int e = gn_check_overlap(y, residual, C, "gn_act_fwd", "residual")) return e;
     YOLO_REQUIRE((uintptr_t)workspace % 16 == 0, "gn_act_fwd: workspace is not 16-byte aligned");
     if (ws_bytes < yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype))
         return fail(YOLO_E_WORKSPACE, "gn_act_fwd: workspace of %zu bytes, %zu needed", ws_bytes,
@@ -1202,7 +1223,7 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
         hipLaunchKernelGGL((gn_sums_kernel<unsigned short>), grid, dim3(GN_THREADS), 0, st, p);
     else
         hipLaunchKernelGGL((gn_sums_kernel<float>), grid, dim3(GN_THREADS), 0, st, p);
-    hipLaunchKernelGGL(gn_stats_kernel, dim3(groups, N), dim3(64), 0, st, p);
+    hipLaunchKernelGGL(gn_join_kernel<false>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
     GN_LAUNCH(gn_apply_kernel, grid, st, p);
     YOLO_CHECK_HIP(hipGetLastError());
     return YOLO_OK;
@@ -1218,6 +1239,8 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
     if (int e = gn_check_view(x, x, N, C, es, "gn_act_bwd", "x")) return e;
     if (int e = gn_check_view(dy, x, N, C, es, "gn_act_bwd", "dy")) return e;
     if (int e = gn_check_view(dx, x, N, C, es, "gn_act_bwd", "dx")) return e;
+    if (int e = gn_check_overlap(dx, x, C, "gn_act_bwd", "x")) return e;
+    if (int e = gn_check_overlap(dx, dy, C, "gn_act_bwd", "dy")) return e;
     YOLO_REQUIRE((uintptr_t)workspace % 16 == 0, "gn_act_bwd: workspace is not 16-byte aligned");
     if (ws_bytes < yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype))
         return fail(YOLO_E_WORKSPACE, "gn_act_bwd: workspace of %zu bytes, %zu needed", ws_bytes,
@@ -1257,7 +1280,7 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
     }
     const dim3 grid = gn_grid(p, es);
     GN_LAUNCH(gn_bwd_sums_kernel, grid, st, p);
-    hipLaunchKernelGGL(gn_bwd_terms_kernel, dim3(groups, N), dim3(256), 0, st, p);
+    hipLaunchKernelGGL(gn_join_kernel<true>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
     GN_LAUNCH(gn_bwd_apply_kernel, grid, st, p);
     hipLaunchKernelGGL(gn_bwd_params_kernel, params_grid, dim3(256), 0, st, p);
     YOLO_CHECK_HIP(hipGetLastError());

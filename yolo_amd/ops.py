@@ -39,6 +39,11 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _stream_of(dev: int) -> int:
+    """_stream() where the current device is known already."""
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
@@ -446,7 +451,7 @@ def gn_workspace_bytes(N: int, H: int, W: int, C: int, groups: int, dtype: torch
 
 def _gn_views(what: str, groups: int, act: str, views, vectors, stats: torch.Tensor, workspace: torch.Tensor):
     """Checks of a group-norm call (single-image calls take a few microseconds on the GPU: these stay cheap); returns the
-    views' structs, the activation's code and the dtype's."""
+    views' structs, batch, channels, the codes of activation and dtype, and the stream."""
     (_, first), dt = views[0], views[0][1].buf.dtype
     N, C = first.buf.shape[0], first.C
     dev = first.buf.get_device()
@@ -481,7 +486,7 @@ def _gn_views(what: str, groups: int, act: str, views, vectors, stats: torch.Ten
     code = ACTIVATIONS.get(act)
     if code is None:
         raise ValueError(f"{what}: activation {act!r} (one of {', '.join(ACTIVATIONS)})")
-    return structs, N, C, code, dtype_code(dt)
+    return structs, N, C, code, dtype_code(dt), _stream_of(dev)
 
 
 def gn_act_fwd(x: View, gamma: torch.Tensor, beta: torch.Tensor, y: View, stats: torch.Tensor, workspace: torch.Tensor, *,
@@ -491,10 +496,10 @@ def gn_act_fwd(x: View, gamma: torch.Tensor, beta: torch.Tensor, y: View, stats:
     gn_act_bwd.  ``act``: "leaky" with ``slope`` in [0, 1] (1: no activation, 0: ReLU) or "silu".  ``y`` may be ``x`` or
     ``residual`` (each element is read before it is written); f32 or bf16, sums in f32 / f64."""
     views = (("x", x), ("y", y)) if residual is None else (("x", x), ("y", y), ("residual", residual))
-    v, N, C, code, dt = _gn_views("gn_act_fwd", groups, act, views, (("gamma", gamma), ("beta", beta)), stats, workspace)
+    v, N, C, code, dt, stream = _gn_views("gn_act_fwd", groups, act, views, (("gamma", gamma), ("beta", beta)), stats, workspace)
     check(lib().yolo_gn_act_fwd(v[0], gamma.data_ptr(), beta.data_ptr(), None if residual is None else v[2], v[1],
                                 stats.data_ptr(), N, C, groups, eps, code, slope, dt, workspace.data_ptr(),
-                                workspace.numel() * workspace.element_size(), _stream()), "yolo_gn_act_fwd")
+                                workspace.numel() * workspace.element_size(), stream), "yolo_gn_act_fwd")
 
 
 def gn_act_bwd(dy: View, x: View, gamma: torch.Tensor, beta: torch.Tensor, stats: torch.Tensor, dx: View,
@@ -502,11 +507,11 @@ def gn_act_bwd(dy: View, x: View, gamma: torch.Tensor, beta: torch.Tensor, stats
                slope: float = 0.1) -> None:
     """Backward of gn_act_fwd from its input and ``stats``: dx, dgamma [C], dbeta [C] (f32, overwritten).  The residual's
     gradient is dy itself.  ``dx`` may be ``dy`` or ``x``."""
-    v, N, C, code, dt = _gn_views("gn_act_bwd", groups, act, (("x", x), ("dy", dy), ("dx", dx)),
+    v, N, C, code, dt, stream = _gn_views("gn_act_bwd", groups, act, (("x", x), ("dy", dy), ("dx", dx)),
                                   (("gamma", gamma), ("beta", beta), ("dgamma", dgamma), ("dbeta", dbeta)), stats, workspace)
     check(lib().yolo_gn_act_bwd(v[1], v[0], gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), v[2], dgamma.data_ptr(),
                                 dbeta.data_ptr(), N, C, groups, code, slope, dt, workspace.data_ptr(),
-                                workspace.numel() * workspace.element_size(), _stream()), "yolo_gn_act_bwd")
+                                workspace.numel() * workspace.element_size(), stream), "yolo_gn_act_bwd")
 
 
 def wgrad_workspace_bytes(M: int, cin: int, cout: int, k: int) -> int:
