@@ -992,9 +992,9 @@ def grad_table(tensors: Sequence[torch.Tensor]) -> GradTable:
     spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
     if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
         raise ValueError("grad_table: two tensors share memory (a shared gradient is listed once)")
-    # runs of a workgroup: 16384 elements, shorter where the whole set would not give each CU eight
+    # runs of a workgroup: 16384 elements, down to 4096 where the whole set would not give each CU eight
     total = sum(t.numel() for t in tensors)
-    run = max(1024, min(16384, -(-total // 2048) // 1024 * 1024))
+    run = max(4096, min(16384, total // 2048 // 1024 * 1024))
     rows, first = [], [0]
     for i, t in enumerate(tensors):
         n, es = t.numel(), t.element_size()
@@ -1023,23 +1023,26 @@ def grad_norm(table: GradTable, norms: torch.Tensor, workspace: torch.Tensor, *,
               per_tensor: bool = False, max_norm: float = 0.0, coefs: Optional[torch.Tensor] = None) -> None:
     """norms [1] <- the norm (1, 2 or inf) of all the table's tensors together, or [n_tensors] <- of each; coefs, of the same
     length, <- min(1, max_norm / (norm + 1e-6)).  Nothing is read back to the host."""
-    _require_cuda(table.blocks, "grad_norm")
-    n, dev = table.n_tensors if per_tensor else 1, table.blocks.get_device()
+    n, dev = len(table.tensors) if per_tensor else 1, table.blocks.get_device()
+    if dev != torch.cuda.current_device():
+        _require_cuda(table.blocks, "grad_norm")
     _check_norms(norms, n, "grad_norm: norms", dev)
     _check_norms(coefs, n, "grad_norm: coefs", dev)
     if workspace.get_device() != dev:
         _require_cuda(workspace, "grad_norm: workspace")
     check(lib().yolo_grad_norm(table.blocks.data_ptr(), table.n_blocks, table.first.data_ptr() if per_tensor else None,
-                               table.n_tensors, norm_type, max_norm, norms.data_ptr(),
-                               None if coefs is None else coefs.data_ptr(), workspace.data_ptr(),
-                               workspace.numel() * workspace.element_size(), _stream()), "yolo_grad_norm")
+                               n, norm_type, max_norm, norms.data_ptr(), None if coefs is None else coefs.data_ptr(),
+                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_of(dev)),
+          "yolo_grad_norm")
 
 
 def grad_scale(table: GradTable, coefs: torch.Tensor, *, per_tensor: bool = False) -> None:
     """Multiply the table's tensors by coefs [1], or each by its own of coefs [n_tensors], in place."""
-    _require_cuda(table.blocks, "grad_scale")
-    _check_norms(coefs, table.n_tensors if per_tensor else 1, "grad_scale: coefs", table.blocks.get_device())
-    check(lib().yolo_grad_scale(table.blocks.data_ptr(), table.n_blocks, coefs.data_ptr(), int(per_tensor), _stream()),
+    dev = table.blocks.get_device()
+    if dev != torch.cuda.current_device():
+        _require_cuda(table.blocks, "grad_scale")
+    _check_norms(coefs, len(table.tensors) if per_tensor else 1, "grad_scale: coefs", dev)
+    check(lib().yolo_grad_scale(table.blocks.data_ptr(), table.n_blocks, coefs.data_ptr(), int(per_tensor), _stream_of(dev)),
           "yolo_grad_scale")
 
 
@@ -1098,5 +1101,5 @@ def sgd_step_clipped(param: torch.Tensor, grad: torch.Tensor, mom: torch.Tensor,
     _check_norms(coefs, table.n_tensors if per_tensor else 1, "sgd_step_clipped: coefs", dev)
     check(lib().yolo_sgd_step_clipped(param.data_ptr(), grad.data_ptr(), mom.data_ptr(), table.blocks.data_ptr(),
                                       table.n_blocks, lr0, wd0, lr1, wd1, momentum, None if coefs is None else coefs.data_ptr(),
-                                      int(per_tensor), -1.0 if clip_value is None else clip_value, _stream()),
+                                      int(per_tensor), -1.0 if clip_value is None else clip_value, _stream_of(dev)),
           "yolo_sgd_step_clipped")

@@ -47,6 +47,9 @@ class GradientClipper:
     def measure(self) -> Optional[torch.Tensor]:
         """The norms the clipping goes by ([1] or [n_tensors], overwritten by the next call; ``coefs`` has the factors);
         None for "value".  The gradients are only read."""
+        return self._measure()
+
+    def _measure(self) -> Optional[torch.Tensor]:
         if self.clip_type == "value":
             return None
         ops.grad_norm(self.table, self.norms, self._ws, norm_type=self.norm_type, per_tensor=self.per_tensor,
@@ -56,7 +59,7 @@ class GradientClipper:
     @ops.on_own_device
     def clip_(self) -> Optional[torch.Tensor]:
         """measure(), then the gradients clipped in place."""
-        norms = self.measure()
+        norms = self._measure()
         if self.clip_type == "value":
             ops.grad_clamp(self.table, self.clip_value)
         else:
