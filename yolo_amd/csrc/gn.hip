@@ -835,7 +835,8 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
             gn_store<ST>(y, to, GnVec<E>::pack(f));
         };
         if (res) {  // the residual of the next vectors is on its way while the last ones are finished
-            constexpr int AHEAD = NV > 16 ? 2 : 4;
+            // above 16 vectors more would not stay in registers (64 x 52 x 52 x 256: 57.7 us with 1, 60.4 with 2, 65.7 with 4)
+            constexpr int AHEAD = NV > 16 ? 1 : 4;
             GnWalk<1> ahead(p, t, cb, {&p.r});
             GnCursor<1> c = gn_again<1>(p, t, cb, {&p.y});
             u32x4 r[AHEAD];
@@ -1100,11 +1101,11 @@ static dim3 gn_grid(const GnParams& p, int es) {
     return dim3(p.chunks, (vecs + p.VS - 1) / p.VS, p.N);
 }
 
-// A call that moves more than this leaves little of use in the 256 MB cache in front of HBM; its loads and stores go past the caches,
-// and what the first pass over x has left there stays for the second.  Measured (bf16, us): 64 x 208 x 208 x 64 forward 230 -> 193,
-// backward 347 -> 306; 64 x 52 x 52 x 256 forward 47 -> 36; 64 x 13 x 13 x 1024 backward (66 MB) 23.0 -> 21.8; below that it loses
-// (16 x 104 x 104 x 64 forward: 31.9 -> 33.4 us).  Only where a workgroup's stores are whole cache lines: narrower slabs share
-// them, and lose a factor of two and more.
+// A call that moves more than this leaves little of use in the 256 MB cache in front of HBM; its loads and stores go past the
+// caches, and what the first pass over x has left there stays for the second.  Measured (bf16, us): 64 x 208 x 208 x 64 forward
+// 230 -> 193, backward 347 -> 306; 64 x 52 x 52 x 256 forward 47 -> 36; 64 x 13 x 13 x 1024 backward (66 MB) 23.0 -> 21.8; the
+// one that lost, 16 x 104 x 104 x 128 forward (88 MB): 31.9 -> 33.4.  A network's training step takes the same time with either.
+// Only where a workgroup's stores are whole cache lines: narrower slabs share them, and lose a factor of two and more.
 constexpr long long GN_STREAM_BYTES = 64ll << 20;
 static int gn_stream_rule(const GnParams& p, int es, int tensors) {
     return (long long)tensors * p.N * p.HW * p.C * es >= GN_STREAM_BYTES;
