@@ -10,6 +10,7 @@ import math
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -793,7 +794,6 @@ def resample_tables(in_size: int, out_size: int, device) -> Tuple[torch.Tensor, 
     key = (in_size, out_size, str(device))
     hit = _RESAMPLE_TABLES.get(key)
     if hit is None:
-        import numpy as np
         scale = in_size / out_size
         filterscale = max(scale, 1.0)
         support = 1.0 * filterscale
@@ -995,15 +995,21 @@ def grad_table(tensors: Sequence[torch.Tensor]) -> GradTable:
     # runs of a workgroup: 16384 elements, down to 4096 where the whole set would not give each CU eight
     total = sum(t.numel() for t in tensors)
     run = max(4096, min(16384, total // 2048 // 1024 * 1024))
-    rows, first = [], [0]
-    for i, t in enumerate(tensors):
-        n, es = t.numel(), t.element_size()
-        rows += [(t.data_ptr() + o * es, min(run, n - o), i, dtype_code(t.dtype), 0) for o in range(0, n, run)]
-        first.append(len(rows))
+    counts = np.array([t.numel() for t in tensors], np.int64)
+    runs = -(-counts // run)
+    first = np.concatenate([[0], np.cumsum(runs)])
+    owner = np.repeat(np.arange(len(tensors)), runs)
+    begin = (np.arange(first[-1]) - first[owner]) * run     # a run's first element in its tensor
+    sizes = np.array([t.element_size() for t in tensors], np.int64)
+    blocks = np.zeros(max(1, len(owner)), np.dtype(GradBlock))
+    rows = blocks[:len(owner)]
+    rows["ptr"] = np.array([t.data_ptr() for t in tensors], np.uint64)[owner] + (begin * sizes[owner]).astype(np.uint64)
+    rows["count"] = np.minimum(run, counts[owner] - begin)
+    rows["tensor"] = owner
+    rows["dtype"] = np.array([dtype_code(t.dtype) for t in tensors])[owner]
     dev = tensors[0].device
-    raw = (GradBlock * max(1, len(rows)))(*rows)
-    blocks = torch.frombuffer(bytearray(bytes(raw)), dtype=torch.uint8).to(dev)
-    return GradTable(blocks, len(rows), torch.tensor(first, dtype=torch.int32).to(dev), tensors)
+    return GradTable(torch.from_numpy(blocks.view(np.uint8)).to(dev), len(rows),
+                     torch.from_numpy(first.astype(np.int32)).to(dev), tensors)
 
 
 def grad_norm_workspace_bytes(table: GradTable) -> int:
@@ -1064,20 +1070,25 @@ class SgdClipTable:
 def sgd_clip_table(segments: Sequence[Tuple[int, int, int]], device) -> SgdClipTable:
     """Block table of ``sgd_step_clipped`` for ``segments`` = (first element, count, group) runs of the arenas, one for each
     tensor in the order of the clip factors; no element is in two of them."""
-    rows, spans = [], []
+    spans, parts = [], []
     for tensor, (first, count, group) in enumerate(segments):
         if first < 0 or count < 0 or group not in (0, 1) or first + count >= 1 << 31:
             raise ValueError(f"sgd_clip_table: segment ({first}, {count}, {group})")
+        if not count:
+            continue
         spans.append((first, first + count))
-        at, end = first, first + count
-        while at < end:   # runs end at multiples of 4096 elements, so that all but a segment's first begin aligned
-            n = min(end, (at // 4096 + 1) * 4096) - at
-            rows.append((at, n, group, tensor))
-            at += n
-    spans = sorted(s for s in spans if s[0] < s[1])
+        # runs end at multiples of 4096 elements, so that all but a segment's first begin aligned
+        ends = np.arange(first // 4096 + 1, (first + count + 4095) // 4096 + 1) * 4096
+        ends[-1] = first + count
+        begins = np.concatenate([[first], ends[:-1]])
+        part = np.empty((len(ends), 4), np.int32)
+        part[:, 0], part[:, 1], part[:, 2], part[:, 3] = begins, ends - begins, group, tensor
+        parts.append(part)
+    spans.sort()
     if not spans or any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
         raise ValueError("sgd_clip_table: no elements, or an element in two segments")
-    return SgdClipTable(torch.tensor(rows, dtype=torch.int32, device=device).contiguous(), len(rows), len(segments), spans[-1][1])
+    rows = np.concatenate(parts)
+    return SgdClipTable(torch.from_numpy(rows).to(device), len(rows), len(segments), spans[-1][1])
 
 
 def sgd_step_clipped(param: torch.Tensor, grad: torch.Tensor, mom: torch.Tensor, table: SgdClipTable, lr0: float, wd0: float,
