@@ -175,6 +175,30 @@ def test_backward(cuda, shape, dtype, act, slope):
     _check_backward(x, dy, gamma, beta, stats, G, act, slope, _backward(cuda, x, dy, gamma, beta, stats, G, act, slope, (1, 0, 2)))
 
 
+# images whose slabs are held in part: each thread's last pixels in LDS or read again; few and many of them, slabs of 80 bytes
+TALL = [(128, 33, 35, 64, 32), (128, 43, 41, 64, 16), (130, 40, 40, 40, 5), (256, 64, 62, 16, 1)]
+
+
+@pytest.mark.parametrize("act,slope", [("leaky", 0.1), ("silu", 0.0)], ids=["leaky", "silu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", TALL, ids=ids)
+def test_backward_of_tall_slabs(cuda, shape, dtype, act, slope):
+    from yolo_amd import ops
+    x, _, dy, gamma, beta = _inputs(shape, dtype, seed=4)
+    N, H, W, C, G = shape
+    stats = torch.stack(_ref_stats(x, G)).float()
+    got = _backward(cuda, x, dy, gamma, beta, stats, G, act, slope, (1, 0, 2))
+    _check_backward(x, dy, gamma, beta, stats, G, act, slope, got)
+    for over_x in (False, True):   # in place: the same bits
+        xv, dyv = _view(x, cuda, 1), _view(dy, cuda, 1)
+        dg, db = torch.empty(C, device=cuda), torch.empty(C, device=cuda)
+        ws = torch.empty(ops.gn_workspace_bytes(N, H, W, C, G, dtype), dtype=torch.uint8, device=cuda)
+        out = xv if over_x else dyv
+        ops.gn_act_bwd(dyv, xv, gamma.to(cuda), beta.to(cuda), stats.to(cuda), out, dg, db, ws, groups=G, act=act, slope=slope)
+        for a, b in zip((out.interior(), dg, db), got):
+            assert torch.equal(a.double().cpu(), b)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_views_slices_halos_and_buffers_used_twice(cuda, dtype):
     """Channel slices of wider buffers, in-place outputs: the same bits as separate buffers, nothing else written."""
@@ -208,7 +232,8 @@ def test_views_slices_halos_and_buffers_used_twice(cuda, dtype):
         assert torch.equal(dg.double().cpu(), dg0) and torch.equal(db.double().cpu(), db0)
 
 
-@pytest.mark.parametrize("shape", [(2, 13, 13, 64, 32), (1, 40, 40, 32, 8), (2, 208, 104, 16, 2)], ids=ids)
+@pytest.mark.parametrize("shape", [(2, 13, 13, 64, 32), (1, 40, 40, 32, 8), (2, 208, 104, 16, 2), (128, 43, 41, 64, 16)],
+                         ids=ids)
 def test_the_side_of_the_kink_is_exact(cuda, shape):
     """Leaky derivative next to t = 0: every t is within a few roundings of zero, so that fp32 arithmetic takes the wrong side for
     many of them; a wrong one moves dx by 0.9 |gamma d r|, far above the tolerance.  t == 0 takes the slope."""

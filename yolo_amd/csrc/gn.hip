@@ -522,10 +522,10 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_sums_kernel(const GnPara
     }
 }
 
-// dgamma, dbeta: the images' sums.  A workgroup has 32 of the 2 C columns (d sums, then d * xh sums) and eight rows at a time.
-__global__ void __launch_bounds__(256) gn_bwd_params_kernel(const GnParams p) {
-    __shared__ double red[8][32];
-    const int col = threadIdx.x & 31, row = threadIdx.x >> 5, i = blockIdx.x * 32 + col;
+// dgamma, dbeta: the images' sums.  A workgroup has 32 of the 2 C columns (d sums, then d * xh sums), the i-th such set of them,
+// and eight rows at a time.
+__device__ __forceinline__ void gn_params(const GnParams& p, int set, double (*red)[32]) {
+    const int col = threadIdx.x & 31, row = threadIdx.x >> 5, i = set * 32 + col;
     double a = 0.0;
     if (i < 2 * p.C)
 #pragma unroll 8
@@ -539,16 +539,26 @@ __global__ void __launch_bounds__(256) gn_bwd_params_kernel(const GnParams p) {
         else
             p.dgamma[i - p.C] = (float)a;
     }
+    __syncthreads();
+}
+__global__ void __launch_bounds__(GN_THREADS) gn_bwd_params_kernel(const GnParams p) {
+    __shared__ double red[8][32];
+    gn_params(p, blockIdx.x, red);
 }
 
 // ------------------------------------------------------------------------------------------------ backward, output
-// dx = d * scale - (x - mean) * (r r B) - r A, four pixels at a time.
+// dx = d * scale - (x - mean) * (r r B) - r A, four pixels at a time.  The first plane of the grid sums dgamma and dbeta: a launch
+// of its own for them is 3 us.
 template <typename E, int ACT>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_apply_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
     __shared__ __attribute__((aligned(16))) float lds[4 * GN_THREADS * V];
+    if (blockIdx.z == 0) {
+        for (int set = blockIdx.y * p.chunks + blockIdx.x; set * 32 < 2 * p.C; set += p.chunks * gridDim.y) gn_params(p, set, (double (*)[32])lds);
+        return;
+    }
     const GnLane l = gn_lane<E>(p);
-    const int n = p.N - 1 - blockIdx.z, chunk = p.chunks - 1 - blockIdx.x, S = p.VS * V;
+    const int n = p.N - blockIdx.z, chunk = p.chunks - 1 - blockIdx.x, S = p.VS * V;
     const int first = chunk * p.chunk, last = min(first + p.chunk, p.HW);
     const float* mine = lds + (l.c - blockIdx.y * S);
     gn_stage(lds, p, n, blockIdx.y * S, S);
@@ -869,9 +879,14 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
 // The backward pass the same way: x and dy in registers, the slab's sums per channel (they are also the image's share of dgamma
 // and dbeta), the group's two terms, dx.  Four channels at a time, so that the constants of a channel stay few.  In this form
 //   t = (x - mean) * (gamma r) + beta,   dx = d * (gamma r) - (x - mean) * (r r B) - r A.
-template <typename E, int ACT, int NV>
+//
+// TALL: slabs that do not fit.  A thread's first NV pairs of vectors are in registers, the next GN_KEPT in LDS, and what is left
+// is read again for dx; those beyond NV are summed first, eight channels at a time, as long as the registers are free.
+constexpr int GN_KEPT = 4;
+template <typename E, int ACT, int NV, bool TALL = false>
 __global__ void __launch_bounds__(1024) gn_whole_bwd_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N, HALVES = V / 4;
+    __shared__ u32x4 kept[TALL ? GN_KEPT : 1][2][TALL ? 1024 : 1];
     enum { MEAN, R, GAMMA, BETA, C0, C1, KINDS };
     __shared__ float part[2][GN_WAVES][GN_SLAB];
     __shared__ float chan[2][GN_SLAB];
@@ -893,6 +908,38 @@ __global__ void __launch_bounds__(1024) gn_whole_bwd_kernel(const GnParams p) {
     }
     const char* xp = p.x.p + n * p.x.img;
     const char* dp = p.dy.p + n * p.dy.img;
+    float sd8[V], sx8[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) sd8[e] = sx8[e] = 0.f;
+    const int more = TALL ? max(t.count - NV, 0) : 0;
+    if constexpr (TALL) {
+        __syncthreads();
+        const GnConst<V> k(&of[0][0] + t.cs, GN_SLAB);
+        const float near = gn_near<V>(k.beta);
+        GnCursor<2> c(t.first + NV * t.step, t.step, p.W, cb, {&p.x, &p.dy});
+        int i = 0;
+        gn_pipelined<2, 2>(
+            more,
+            [&](u32x4* r) {
+                r[0] = gn_load(xp, c.at[0]);
+                r[1] = gn_load(dp, c.at[1]);
+                c.next();
+            },
+            [&](const u32x4* r) {
+                if (i < GN_KEPT) {
+                    kept[i][0][threadIdx.x] = r[0];
+                    kept[i][1][threadIdx.x] = r[1];
+                }
+                ++i;
+                float xm[V], a[V];
+                gn_grads<E, ACT>(r[0], r[1], k, near, &of[0][0], t.cs, GN_SLAB, p.slope, xm, a);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    sd8[e] += a[e];
+                    sx8[e] = fmaf(a[e], xm[e], sx8[e]);
+                }
+            });
+    }
     u32x4 x[NV], d[NV];
     gn_with_stream(p.stream, [&](auto st) {
         GnWalk<2> walk(p, t, cb, {&p.x, &p.dy});
@@ -914,7 +961,12 @@ __global__ void __launch_bounds__(1024) gn_whole_bwd_kernel(const GnParams p) {
         const int cs = t.cs + 4 * h;
         const GnConst<4> k(&of[0][0] + cs, GN_SLAB);
         const float near = gn_near<4>(k.beta);
-        float sd[4] = {0.f, 0.f, 0.f, 0.f}, sx[4] = {0.f, 0.f, 0.f, 0.f};
+        float sd[4], sx[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            sd[e] = sd8[4 * h + e];
+            sx[e] = sx8[4 * h + e];
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (i < t.most) {  // where the thread has no pixel dy is zero
@@ -1000,6 +1052,42 @@ __global__ void __launch_bounds__(1024) gn_whole_bwd_kernel(const GnParams p) {
             c.next();
         }
     });
+    if constexpr (TALL) {
+        const GnConst<V> k(&of[0][0] + t.cs, GN_SLAB);
+        const float near = gn_near<V>(k.beta);
+        float k0[V], k1[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            k0[e] = of[C0][t.cs + e];
+            k1[e] = of[C1][t.cs + e];
+        }
+        gn_with_stream(p.stream, [&](auto st) {
+            constexpr int ST = decltype(st)::value;
+            const int there = min(more, GN_KEPT);
+            GnCursor<1> cy(t.first + NV * t.step, t.step, p.W, cb, {&p.y});
+            GnCursor<2> c(t.first + (NV + there) * t.step, t.step, p.W, cb, {&p.x, &p.dy});
+            auto put = [&](const u32x4* r) {
+                float xm[V], a[V];
+                gn_grads<E, ACT>(r[0], r[1], k, near, &of[0][0], t.cs, GN_SLAB, p.slope, xm, a);
+#pragma unroll
+                for (int e = 0; e < V; ++e) a[e] = fmaf(a[e], k.scale[e], fmaf(xm[e], k1[e], k0[e]));
+                gn_store<ST>(y, cy.at[0], GnVec<E>::pack(a));
+                cy.next();
+            };
+            for (int i = 0; i < there; ++i) {
+                const u32x4 r[2] = {kept[i][0][threadIdx.x], kept[i][1][threadIdx.x]};
+                put(r);
+            }
+            gn_pipelined<2, 2>(
+                more - there,
+                [&](u32x4* r) {
+                    r[0] = gn_load<ST>(xp, c.at[0]);
+                    r[1] = gn_load<ST>(dp, c.at[1]);
+                    c.next();
+                },
+                put);
+        });
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -1031,7 +1119,7 @@ static GnTensor gn_tensor(const yolo_view* v, int es) {
 
 static int gn_check_shape(int N, int C, int groups, int act, float slope, int dtype, const char* op) {
     YOLO_REQUIRE(dtype == YOLO_F32 || dtype == YOLO_BF16, "%s: dtype %d", op, dtype);
-    YOLO_REQUIRE(N > 0 && N <= 65535, "%s: batch %d (1 to 65535)", op, N);
+    YOLO_REQUIRE(N > 0 && N <= 65534, "%s: batch %d (1 to 65534)", op, N);
     YOLO_REQUIRE(C > 0 && C % 8 == 0 && C <= 65536, "%s: %d channels (a multiple of 8, at most 65536)", op, C);
     YOLO_REQUIRE(groups > 0 && C % groups == 0, "%s: %d groups do not divide %d channels", op, groups, C);
     YOLO_REQUIRE(act == YOLO_ACT_LEAKY || act == YOLO_ACT_SILU, "%s: activation %d", op, act);
@@ -1063,9 +1151,15 @@ static void gn_split(GnParams& p, int es) {
 //   narrower (to 32 B) for 256 workgroups        16 x 52 x 52 x 256 forward 16.2 with 32 B, 17.5 with 64 B, 24 with 128 B
 //   64 B so that it fits, no less                64 x 104 x 104 x 128 forward 102 with 32 B, in chunks 97; one image 33 and 18
 // Forward a thread takes up to 11 vectors before the workgroup gets more waves (64 x 26 x 26 x 512: 17.8 us with 8 waves of 11, 23.3
-// with 16 of 6); backward it has two tensors' vectors, and spills above 8.
+// with 16 of 6); backward it has two tensors' vectors, and spills above 8.  Taller slabs are then held in part, at 128 B a pixel,
+// where the CUs, one slab each, are busy (backward):
+//   half of the CUs and more, up to 32 vectors   64 x 52 x 52 x 256 68.0, in chunks 83;  32 x 52 x 52 x 256 44, in chunks 52;  16 images
+//                                                37 and 32;  64 x 40 x 40 x 256 41, with 64 B whole 64
+//   all of them, up to 64 vectors                64 x 76 x 76 x 256 150, in chunks 161;  64 x 76 x 76 x 128 (128 slabs) 91 and 87
+//   several slabs each, the last round not empty 96 x 52 x 52 x 256 (384 slabs) 110, in chunks 117;  80 images (320) 104 and 99
 struct GnWhole {
     int VS, waves, NV;
+    bool tall;
 };
 static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out) {
     const int V = 16 / es, vecs = p.C / V;
@@ -1077,9 +1171,17 @@ static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out
     auto fit = [&](int vs) { return vs < uv ? uv : (vs < most ? vs : most) / uv * uv; };  // whole units, about vs vectors
     auto blocks = [&](int vs) { return (long long)p.N * ((vecs + vs - 1) / vs); };
     auto nv = [&](int vs, int waves) { return (p.HW + waves * (64 / vs) - 1) / (waves * (64 / vs)); };
+    out->tall = false;
     int VS = fit(16);
     if (blocks(VS) < 512 || nv(VS, GN_WAVES) > nv_most) VS = fit(8);
-    if (nv(VS, GN_WAVES) > nv_most) VS = fit(4);
+    const long long there = blocks(VS), rounds = (there + 255) / 256;  // a tall slab takes a CU of its own
+    const int tall = nv(VS, GN_WAVES);
+    const bool busy = there <= 256 ? there >= (tall <= 32 ? 128 : 256) : there * 10 >= rounds * 256 * 7;
+    if (backward && tall > nv_most && tall <= 64 && (VS % 8 == 0 || VS == vecs) && busy) {
+        *out = GnWhole{VS, GN_WAVES, tall, true};
+        return true;
+    }
+    if (tall > nv_most) VS = fit(4);
     if (nv(VS, GN_WAVES) > nv_most) return false;
     if (blocks(VS) < 256 && VS > 4) VS = fit(4);
     if (blocks(VS) < 256 && VS > 2) VS = fit(2);
@@ -1127,29 +1229,23 @@ static void gn_shape(GnParams& p, const yolo_view* x, int N, int C, int groups, 
 
 using namespace yolo;
 
-#define GN_LAUNCH(KERNEL, grid, st, p)                                                                                  \
-    do {                                                                                                                \
-        if (dtype == YOLO_BF16 && act == YOLO_ACT_LEAKY)                                                                \
-            hipLaunchKernelGGL((KERNEL<unsigned short, GN_LEAKY>), grid, dim3(GN_THREADS), 0, st, p);                   \
-        else if (dtype == YOLO_BF16)                                                                                    \
-            hipLaunchKernelGGL((KERNEL<unsigned short, GN_SILU>), grid, dim3(GN_THREADS), 0, st, p);                    \
-        else if (act == YOLO_ACT_LEAKY)                                                                                 \
-            hipLaunchKernelGGL((KERNEL<float, GN_LEAKY>), grid, dim3(GN_THREADS), 0, st, p);                            \
-        else                                                                                                            \
-            hipLaunchKernelGGL((KERNEL<float, GN_SILU>), grid, dim3(GN_THREADS), 0, st, p);                             \
+// KERNEL for the call's type and activation; what follows are its other template arguments
+#define GN_LAUNCH(grid, block, KERNEL, ...)                                                                  \
+    do {                                                                                                     \
+        if (dtype == YOLO_BF16 && act == YOLO_ACT_LEAKY)                                                     \
+            hipLaunchKernelGGL((KERNEL<unsigned short, GN_LEAKY, ##__VA_ARGS__>), grid, block, 0, st, p);    \
+        else if (dtype == YOLO_BF16)                                                                         \
+            hipLaunchKernelGGL((KERNEL<unsigned short, GN_SILU, ##__VA_ARGS__>), grid, block, 0, st, p);     \
+        else if (act == YOLO_ACT_LEAKY)                                                                      \
+            hipLaunchKernelGGL((KERNEL<float, GN_LEAKY, ##__VA_ARGS__>), grid, block, 0, st, p);             \
+        else                                                                                                 \
+            hipLaunchKernelGGL((KERNEL<float, GN_SILU, ##__VA_ARGS__>), grid, block, 0, st, p);              \
     } while (0)
 
-#define GN_WHOLE_CASE(KERNEL, K)                                                                                           \
-    if (w.NV <= K) {                                                                                                       \
-        if (dtype == YOLO_BF16 && act == YOLO_ACT_LEAKY)                                                                   \
-            hipLaunchKernelGGL((KERNEL<unsigned short, GN_LEAKY, K>), grid, dim3(w.waves * 64), 0, st, p);                 \
-        else if (dtype == YOLO_BF16)                                                                                       \
-            hipLaunchKernelGGL((KERNEL<unsigned short, GN_SILU, K>), grid, dim3(w.waves * 64), 0, st, p);                  \
-        else if (act == YOLO_ACT_LEAKY)                                                                                    \
-            hipLaunchKernelGGL((KERNEL<float, GN_LEAKY, K>), grid, dim3(w.waves * 64), 0, st, p);                          \
-        else                                                                                                               \
-            hipLaunchKernelGGL((KERNEL<float, GN_SILU, K>), grid, dim3(w.waves * 64), 0, st, p);                           \
-    } else
+#define GN_WHOLE_CASE(KERNEL, K)                          \
+    if (w.NV <= K)                                        \
+        GN_LAUNCH(grid, dim3(w.waves * 64), KERNEL, K);   \
+    else
 
 // The channels of a vector that always lie in one group: the largest power of two that divides both.
 static int gn_fold(int Cg, int V) {
@@ -1225,7 +1321,7 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
     else
         hipLaunchKernelGGL((gn_sums_kernel<float>), grid, dim3(GN_THREADS), 0, st, p);
     hipLaunchKernelGGL(gn_join_kernel<false>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
-    GN_LAUNCH(gn_apply_kernel, grid, st, p);
+    GN_LAUNCH(grid, dim3(GN_THREADS), gn_apply_kernel);
     YOLO_CHECK_HIP(hipGetLastError());
     return YOLO_OK;
 }
@@ -1262,7 +1358,6 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
     p.slope = leaky_slope;
     p.stream = gn_stream_rule(p, es, 3);
     hipStream_t st = (hipStream_t)stream;
-    const dim3 params_grid((2 * C + 31) / 32);
     GnWhole w;
     if (gn_whole_plan(p, es, true, &w)) {
         p.VS = w.VS;
@@ -1270,20 +1365,23 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
         p.slabs = (p.C * es / 16 + w.VS - 1) / w.VS;
         p.stream = p.stream && w.VS % 8 == 0;  // whole cache lines only
         const dim3 grid((unsigned)(p.slabs * N));
+        if (w.tall)
+            GN_LAUNCH(grid, dim3(1024), gn_whole_bwd_kernel, 8, true);
+        else
         GN_WHOLE_CASE(gn_whole_bwd_kernel, 1)
         GN_WHOLE_CASE(gn_whole_bwd_kernel, 2)
         GN_WHOLE_CASE(gn_whole_bwd_kernel, 4)
         GN_WHOLE_CASE(gn_whole_bwd_kernel, 6)
         GN_WHOLE_CASE(gn_whole_bwd_kernel, 8) { return fail(YOLO_E_ARG, "gn_act_bwd: no kernel for %d vectors", w.NV); }
-        hipLaunchKernelGGL(gn_bwd_params_kernel, params_grid, dim3(256), 0, st, p);
+        hipLaunchKernelGGL(gn_bwd_params_kernel, dim3((2 * C + 31) / 32), dim3(GN_THREADS), 0, st, p);
         YOLO_CHECK_HIP(hipGetLastError());
         return YOLO_OK;
     }
-    const dim3 grid = gn_grid(p, es);
-    GN_LAUNCH(gn_bwd_sums_kernel, grid, st, p);
+    dim3 grid = gn_grid(p, es);
+    GN_LAUNCH(grid, dim3(GN_THREADS), gn_bwd_sums_kernel);
     hipLaunchKernelGGL(gn_join_kernel<true>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
-    GN_LAUNCH(gn_bwd_apply_kernel, grid, st, p);
-    hipLaunchKernelGGL(gn_bwd_params_kernel, params_grid, dim3(256), 0, st, p);
+    ++grid.z;  // dgamma and dbeta
+    GN_LAUNCH(grid, dim3(GN_THREADS), gn_bwd_apply_kernel);
     YOLO_CHECK_HIP(hipGetLastError());
     return YOLO_OK;
 }
