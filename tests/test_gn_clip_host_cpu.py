@@ -19,18 +19,20 @@ def _fwd(x=None, y=None, r=None, N=1, C=64, groups=32, eps=1e-5, act=0, slope=0.
     return code, L.yolo_last_error().decode()
 
 
-def _bwd(dy=None, x=None, dx=None, N=1, C=64, groups=32, act=0, slope=0.1, dtype=1, ws=1 << 30, ptr=4096):
+def _bwd(dy=None, x=None, dx=None, N=1, C=64, groups=32, act=0, slope=0.1, dtype=1, ws=1 << 30, ptr=4096, dgamma=None, dbeta=None):
     L = _lib.lib()
     dy, x, dx = dy or _view(), x or _view(), dx or _view()
-    code = L.yolo_gn_act_bwd(ctypes.byref(dy), ctypes.byref(x), ptr, ptr, ptr, ctypes.byref(dx), ptr, ptr, N, C, groups, act,
-                             slope, dtype, ptr, ws, None)
+    at = lambda i: ptr and ptr + 4096 * i  # noqa: E731
+    dgamma, dbeta = at(3) if dgamma is None else dgamma, at(4) if dbeta is None else dbeta
+    code = L.yolo_gn_act_bwd(ctypes.byref(dy), ctypes.byref(x), at(1), at(2), ptr, ctypes.byref(dx), dgamma, dbeta, N, C, groups,
+                             act, slope, dtype, ptr, ws, None)
     return code, L.yolo_last_error().decode()
 
 
 @pytest.mark.parametrize("call", [_fwd, _bwd], ids=["fwd", "bwd"])
 @pytest.mark.parametrize("kw,says", [
     (dict(ptr=None), "null"), (dict(x=_view(ptr=None)), "null"), (dict(x=_view(H=0)), "expected"), (dict(N=0), "batch"),
-    (dict(N=65536), "batch"), (dict(C=60), "channels"), (dict(C=0), "channels"), (dict(groups=0), "groups"),
+    (dict(N=65535), "batch"), (dict(N=32768, C=32768, groups=32768, x=_view(1, 1, total=32768)), "2^30"), (dict(C=60), "channels"), (dict(C=0), "channels"), (dict(groups=0), "groups"),
     (dict(groups=7), "groups"), (dict(act=2), "activation"), (dict(slope=-0.1), "slope"), (dict(slope=float("nan")), "slope"),
     (dict(dtype=2), "dtype"), (dict(ws=16), "workspace"), (dict(x=_view(at=8)), "slice"), (dict(x=_view(total=68)), "slice"),
     (dict(x=_view(ptr=4100)), "aligned"), (dict(x=_view(H=4096, W=4096, total=64)), "2 GiB")],
@@ -48,6 +50,14 @@ def test_gn_refusals_of_one_direction():
     for kw in (dict(x=wide(0), y=wide(8)), dict(x=wide(64), y=wide(64, 1)), dict(x=wide(128), y=wide(0), r=wide(56))):
         assert "lies over part" in _fwd(**kw)[1]
     assert "lies over part of dy" in _bwd(x=wide(0), dx=wide(64), dy=wide(72))[1]
+    image = 8 * 8 * 64 * 2     # buffers that begin elsewhere: images of one batch, the last byte of a neighbour
+    for at in (image, -image, 2 * image - 16, 16 - 2 * image):
+        assert "lies over part" in _fwd(N=2, x=_view(ptr=1 << 20), y=_view(ptr=(1 << 20) + at))[1]
+        assert "lies over part of dy" in _bwd(N=2, x=_view(ptr=1 << 30), dy=_view(ptr=1 << 20), dx=_view(ptr=(1 << 20) + at))[1]
+    for at in (2 * image, -2 * image):
+        assert _fwd(N=2, x=_view(ptr=1 << 20), y=_view(ptr=(1 << 20) + at), ws=16)[0] == -2
+    for kw in (dict(dgamma=8192), dict(dgamma=3 * 4096), dict(dbeta=8192), dict(dbeta=3 * 4096), dict(dgamma=1 << 16, dbeta=1 << 16)):
+        assert "memory of their own" in _bwd(**kw)[1]
     L = _lib.lib()
     assert L.yolo_gn_workspace_bytes(0, 8, 8, 64, 32, 1) == 0 and L.yolo_gn_workspace_bytes(1, 8, 8, 60, 4, 1) == 0
     assert L.yolo_gn_workspace_bytes(64, 208, 208, 64, 32, 1) > 0

@@ -9,8 +9,11 @@
 //             dbeta = sum over images and pixels of d,  dgamma = the same of d * xh
 //             dx = r * (gamma * d - A - xh * B),  A = sum over the group of gamma * d / M,  B = the same of d * xh
 //
-// Memory-bound: a pass reads or writes 16 bytes per lane, sums are fp32 within a thread (about a pivot where squares would
-// cancel) and fp64 from there on.
+// Memory-bound: some twenty operations for each value of 2 or 4 bytes.  A pass reads or writes 16 bytes per lane, sums are fp32
+// within a thread (about a pivot where squares would cancel) and fp64 from there on.  Two forms, chosen by gn_whole_plan:
+//   whole    a workgroup holds a slab (whole groups) of one image in registers: x and dy are read once, one launch
+//   chunked  an image's slab over many workgroups, with a second pass over x and dy: sums, join, output
+// No atomics and a fixed order of additions: a call gives the same bits each time.
 #include <type_traits>
 
 #include "common.h"
@@ -292,6 +295,8 @@ __device__ __forceinline__ GnLane gn_lane(const GnParams& p) {
 // ------------------------------------------------------------------------------------------------ forward, sums
 // partial[n][chunk][0 / 1][c] = sum of x, of x * x over the chunk's pixels.  A thread sums differences from the first value
 // it sees (fp32; the values of a few dozen pixels differ from it by about their spread), and goes over to fp64 after that.
+// Bound by the read: 64 x 208 x 208 x 64 bf16, 354 MB in 65 us, 5.4 TB/s.  256 threads, at most 128 pixels to a thread: 2048
+// workgroups, so that a CU has the loads of several in flight.
 template <typename E>
 __global__ void __launch_bounds__(GN_THREADS, 5) gn_sums_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
@@ -345,8 +350,8 @@ __global__ void __launch_bounds__(GN_THREADS, 5) gn_sums_kernel(const GnParams p
 }
 
 // The chunks' sums of the groups of about 64 channels of one image, in fp64 and in the chunks' order: lanes are channels, the
-// sixteen waves take the chunks in turn.  Forward: mean and r of a group.  Backward: the image's sums of each channel, and the group's two
-// terms from gamma times them.
+// sixteen waves take the chunks in turn.  Forward: mean and r of a group.  Backward: the image's sums of each channel, and the
+// group's two terms from gamma times them.  Latency-bound, 4 to 5 us.
 constexpr int GN_JOIN = 16;
 template <bool BWD>
 __global__ void __launch_bounds__(GN_JOIN * 64) gn_join_kernel(const GnParams p) {
@@ -406,6 +411,8 @@ __global__ void __launch_bounds__(GN_JOIN * 64) gn_join_kernel(const GnParams p)
 }
 
 // ------------------------------------------------------------------------------------------------ forward, output
+// y = act((x - mean) * (gamma r) + beta) [+ residual], images and chunks in the reverse order of the sums: what was read last is
+// still in the cache in front of HBM.  64 x 208 x 208 x 64 bf16: 709 MB in 123 us, 5.8 TB/s.
 template <typename E, int ACT>
 __global__ void __launch_bounds__(GN_THREADS, 8) gn_apply_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
@@ -465,7 +472,7 @@ __global__ void __launch_bounds__(GN_THREADS, 8) gn_apply_kernel(const GnParams 
 }
 
 // ------------------------------------------------------------------------------------------------ backward, sums
-// partial[n][chunk][0 / 1][c] = sum of d, of d * xh over the chunk's pixels
+// partial[n][chunk][0 / 1][c] = sum of d, of d * xh over the chunk's pixels, two pairs of vectors ahead.  64 x 208 x 208 x 64 bf16: 709 MB in 118 us, 6.0 TB/s.
 template <typename E, int ACT>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_sums_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
@@ -547,14 +554,16 @@ __global__ void __launch_bounds__(GN_THREADS) gn_bwd_params_kernel(const GnParam
 }
 
 // ------------------------------------------------------------------------------------------------ backward, output
-// dx = d * scale - (x - mean) * (r r B) - r A, four pixels at a time.  The first plane of the grid sums dgamma and dbeta: a launch
+// dx = d * scale - (x - mean) * (r r B) - r A, four pixels at a time, images and chunks in the reverse order of the sums (64 x
+// 208 x 208 x 64 bf16: 1063 MB in 178 us, 6.0 TB/s).  The first plane of the grid sums dgamma and dbeta: a launch
 // of its own for them is 3 us.
 template <typename E, int ACT>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_apply_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
     __shared__ __attribute__((aligned(16))) float lds[4 * GN_THREADS * V];
     if (blockIdx.z == 0) {
-        for (int set = blockIdx.y * p.chunks + blockIdx.x; set * 32 < 2 * p.C; set += p.chunks * gridDim.y) gn_params(p, set, (double (*)[32])lds);
+        for (int set = blockIdx.y * p.chunks + blockIdx.x; set * 32 < 2 * p.C; set += p.chunks * gridDim.y)
+            gn_params(p, set, (double (*)[32])lds);
         return;
     }
     const GnLane l = gn_lane<E>(p);
@@ -607,7 +616,9 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_apply_kernel(const GnPar
 // ------------------------------------------------------------------------------------------------ whole images
 // One workgroup holds all pixels of a slab of whole groups of one image in registers, so that x (and dy) are read once: VS
 // vectors of 16 bytes per pixel, 64 / VS pixels next to each other in a wave, NV vectors to a thread.  The statistics are then
-// the two sums of the definition (mean, then squares about it), fp32 in a thread and fp64 between threads.
+// the two sums of the definition (mean, then squares about it), fp32 in a thread and fp64 between threads.  64 x 52 x 52 x 256 bf16
+// with a residual: 266 MB in 57 us, 4.7 TB/s (one round of 256 workgroups that load, add up and store at the same time); one image
+// of 13 x 13 x 1024: 6.4 us, of which a launch and the way to memory and back are most.
 constexpr int GN_SLAB = 128;  // most channels of a slab (at most the threads of the smallest workgroup)
 constexpr int GN_WAVES = 16;
 
@@ -880,8 +891,12 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
 // and dbeta), the group's two terms, dx.  Four channels at a time, so that the constants of a channel stay few.  In this form
 //   t = (x - mean) * (gamma r) + beta,   dx = d * (gamma r) - (x - mean) * (r r B) - r A.
 //
+// 64 x 13 x 13 x 1024 bf16: 66 MB in 18 us, and 3 us for dgamma and dbeta.
+//
 // TALL: slabs that do not fit.  A thread's first NV pairs of vectors are in registers, the next GN_KEPT in LDS, and what is left
-// is read again for dx; those beyond NV are summed first, eight channels at a time, as long as the registers are free.
+// is read again for dx; those beyond NV are summed first, eight channels at a time, as long as the registers are free.  The call on
+// 64 x 52 x 52 x 256 bf16, 12 of a thread's 21 or 22 pairs held, takes 68 us, in chunks 83.  Eight pairs in registers spill a dozen
+// values in bf16 (leaky) and are still no slower than seven or six (68.4, 68.1, 68.7 us; 64 x 38 x 38 x 512: 79.9, 81.2, 80.4).
 constexpr int GN_KEPT = 4;
 template <typename E, int ACT, int NV, bool TALL = false>
 __global__ void __launch_bounds__(1024) gn_whole_bwd_kernel(const GnParams p) {
@@ -1104,11 +1119,14 @@ static int gn_check_view(const yolo_view* v, const yolo_view* like, int N, int C
 }
 
 // An output over an input: all of it in place, or none of it.
-static int gn_check_overlap(const yolo_view* out, const yolo_view* in, int C, const char* op, const char* what) {
-    if (out->ptr != in->ptr || (out->ch_offset == in->ch_offset && out->ch_total == in->ch_total && out->halo == in->halo)) return YOLO_OK;
-    YOLO_REQUIRE(out->ch_total == in->ch_total && out->halo == in->halo &&
-                     (out->ch_offset + C <= in->ch_offset || in->ch_offset + C <= out->ch_offset),
-                 "%s: the output lies over part of %s", op, what);
+static int gn_check_overlap(const yolo_view* out, const yolo_view* in, int N, int C, int es, const char* op, const char* what) {
+    const bool same = out->ch_total == in->ch_total && out->halo == in->halo;
+    if (out->ptr == in->ptr && same &&
+        (out->ch_offset == in->ch_offset || out->ch_offset + C <= in->ch_offset || in->ch_offset + C <= out->ch_offset))
+        return YOLO_OK;
+    auto bytes = [&](const yolo_view* v) { return (uintptr_t)N * (v->H + 2 * v->halo) * (v->W + 2 * v->halo) * v->ch_total * es; };
+    const uintptr_t a = (uintptr_t)out->ptr, b = (uintptr_t)in->ptr;
+    YOLO_REQUIRE(a + bytes(out) <= b || b + bytes(in) <= a, "%s: the output lies over part of %s", op, what);
     return YOLO_OK;
 }
 
@@ -1122,6 +1140,7 @@ static int gn_check_shape(int N, int C, int groups, int act, float slope, int dt
     YOLO_REQUIRE(N > 0 && N <= 65534, "%s: batch %d (1 to 65534)", op, N);
     YOLO_REQUIRE(C > 0 && C % 8 == 0 && C <= 65536, "%s: %d channels (a multiple of 8, at most 65536)", op, C);
     YOLO_REQUIRE(groups > 0 && C % groups == 0, "%s: %d groups do not divide %d channels", op, groups, C);
+    YOLO_REQUIRE(2ll * N * groups < (1ll << 31), "%s: %d images of %d groups (below 2^30 together)", op, N, groups);
     YOLO_REQUIRE(act == YOLO_ACT_LEAKY || act == YOLO_ACT_SILU, "%s: activation %d", op, act);
     YOLO_REQUIRE(act != YOLO_ACT_LEAKY || (slope >= 0.f && slope <= 1.f), "%s: leaky slope %g outside [0, 1]", op, (double)slope);
     return YOLO_OK;
@@ -1153,8 +1172,8 @@ static void gn_split(GnParams& p, int es) {
 // Forward a thread takes up to 11 vectors before the workgroup gets more waves (64 x 26 x 26 x 512: 17.8 us with 8 waves of 11, 23.3
 // with 16 of 6); backward it has two tensors' vectors, and spills above 8.  Taller slabs are then held in part, at 128 B a pixel,
 // where the CUs, one slab each, are busy (backward):
-//   half of the CUs and more, up to 32 vectors   64 x 52 x 52 x 256 68.0, in chunks 83;  32 x 52 x 52 x 256 44, in chunks 52;  16 images
-//                                                37 and 32;  64 x 40 x 40 x 256 41, with 64 B whole 64
+//   half of the CUs and more, up to 32 vectors   64 x 52 x 52 x 256 68.0, in chunks 83;  32 images 44 and 52;  16 images 37 and 32
+//                                                64 x 40 x 40 x 256 41, with 64 B whole 64
 //   all of them, up to 64 vectors                64 x 76 x 76 x 256 150, in chunks 161;  64 x 76 x 76 x 128 (128 slabs) 91 and 87
 //   several slabs each, the last round not empty 96 x 52 x 52 x 256 (384 slabs) 110, in chunks 117;  80 images (320) 104 and 99
 struct GnWhole {
@@ -1276,9 +1295,9 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
     if (int e = gn_check_view(y, x, N, C, es, "gn_act_fwd", "y")) return e;
     if (residual)
         if (int e = gn_check_view(residual, x, N, C, es, "gn_act_fwd", "residual")) return e;
-    if (int e = gn_check_overlap(y, x, C, "gn_act_fwd", "x")) return e;
+    if (int e = gn_check_overlap(y, x, N, C, es, "gn_act_fwd", "x")) return e;
     if (residual)
-        if (int e = gn_check_overlap(y, residual, C, "gn_act_fwd", "residual")) return e;
+        if (int e = gn_check_overlap(y, residual, N, C, es, "gn_act_fwd", "residual")) return e;
     YOLO_REQUIRE((uintptr_t)workspace % 16 == 0, "gn_act_fwd: workspace is not 16-byte aligned");
     if (ws_bytes < yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype))
         return fail(YOLO_E_WORKSPACE, "gn_act_fwd: workspace of %zu bytes, %zu needed", ws_bytes,
@@ -1336,8 +1355,10 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
     if (int e = gn_check_view(x, x, N, C, es, "gn_act_bwd", "x")) return e;
     if (int e = gn_check_view(dy, x, N, C, es, "gn_act_bwd", "dy")) return e;
     if (int e = gn_check_view(dx, x, N, C, es, "gn_act_bwd", "dx")) return e;
-    if (int e = gn_check_overlap(dx, x, C, "gn_act_bwd", "x")) return e;
-    if (int e = gn_check_overlap(dx, dy, C, "gn_act_bwd", "dy")) return e;
+    if (int e = gn_check_overlap(dx, x, N, C, es, "gn_act_bwd", "x")) return e;
+    if (int e = gn_check_overlap(dx, dy, N, C, es, "gn_act_bwd", "dy")) return e;
+    YOLO_REQUIRE(dgamma != dbeta && dgamma != gamma && dgamma != beta && dbeta != gamma && dbeta != beta,
+                 "gn_act_bwd: dgamma and dbeta need memory of their own");
     YOLO_REQUIRE((uintptr_t)workspace % 16 == 0, "gn_act_bwd: workspace is not 16-byte aligned");
     if (ws_bytes < yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype))
         return fail(YOLO_E_WORKSPACE, "gn_act_bwd: workspace of %zu bytes, %zu needed", ws_bytes,
