@@ -34,13 +34,15 @@ class GradientClipper:
 
     def __init__(self, grads: Sequence[torch.Tensor], clip_type: str, clip_value: float, norm_type: float = 2.0):
         self.clip_type, self.clip_value, self.norm_type = _check_clip(clip_type, clip_value, norm_type)
-        self.table = ops.grad_table(grads)
-        self.device = self.table.blocks.device
+        grads = list(grads)
         self.per_tensor = clip_type == "norm"
         self.norms = self.coefs = self._ws = None
-        if clip_type != "value":
-            n = self.table.n_tensors if self.per_tensor else 1
-            self.norms, self.coefs = torch.zeros(n, device=self.device), torch.ones(n, device=self.device)
+        if clip_type != "value" and grads:   # filled by the time the table's synchronous copy is done: any stream may come next
+            n = len(grads) if self.per_tensor else 1
+            self.norms, self.coefs = torch.zeros(n, device=grads[0].device), torch.ones(n, device=grads[0].device)
+        self.table = ops.grad_table(grads)
+        self.device = self.table.blocks.device
+        if self.norms is not None:
             self._ws = torch.empty(ops.grad_norm_workspace_bytes(self.table), dtype=torch.uint8, device=self.device)
 
     @ops.on_own_device
