@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
 
@@ -450,27 +451,33 @@ def gn_workspace_bytes(N: int, H: int, W: int, C: int, groups: int, dtype: torch
     return int(lib().yolo_gn_workspace_bytes(N, H, W, C, groups, dtype_code(dtype)))
 
 
+_pack_view = struct.Struct("Piiiii4x").pack   # a YoloView's bytes, at a quarter of the cost of the ctypes structure
+
+
 def _gn_views(what: str, groups: int, act: str, views, vectors, stats: torch.Tensor, workspace: torch.Tensor):
     """Checks of a group-norm call (single-image calls take a few microseconds on the GPU: these stay cheap); returns the
     views' structs, batch, channels, the codes of activation and dtype, and the stream."""
-    (_, first), dt = views[0], views[0][1].buf.dtype
-    N, C = first.buf.shape[0], first.C
-    dev = first.buf.get_device()
+    first = views[0][1]
+    dt, C, dev = first.buf.dtype, first.C, first.buf.get_device()
     if dev < 0 or dev != torch.cuda.current_device():
         _require_cuda(first.buf, f"{what}: {views[0][0]}")
-    structs = []
+    N, structs = -1, []
     for name, v in views:
-        buf = v.buf
+        buf, H, W, halo = v.buf, v.H, v.W, v.halo
         if buf.get_device() != dev:
             _require_cuda(buf, f"{what}: {name}")
         # the kernels address the view from its struct alone: the buffer behind it has to be what the struct says
         shape = buf.shape
-        if len(shape) != 4 or not buf.is_contiguous() or shape[1] != v.H + 2 * v.halo or shape[2] != v.W + 2 * v.halo:
-            raise ValueError(f"{what}: {name}: a {v.H} x {v.W} view with halo {v.halo} does not describe its "
-                             f"{tuple(shape)} buffer")
-        if buf.dtype != dt or shape[0] != N or v.C != C:
-            raise ValueError(f"{what}: {name} is {shape[0]} x {v.C} channels of {buf.dtype}, expected {N} x {C} of {dt}")
-        structs.append(YoloView(buf.data_ptr(), v.H, v.W, v.halo, shape[3], v.ch_offset))
+        if len(shape) != 4 or not buf.is_contiguous():
+            raise ValueError(f"{what}: {name}: needs a contiguous [N, H, W, C] buffer, not {tuple(shape)}")
+        n, rows, cols, total = shape
+        if rows != H + 2 * halo or cols != W + 2 * halo:
+            raise ValueError(f"{what}: {name}: a {H} x {W} view with halo {halo} does not describe its {tuple(shape)} buffer")
+        if N < 0:
+            N = n
+        if n != N or v.C != C or buf.dtype != dt:
+            raise ValueError(f"{what}: {name} is {n} x {v.C} channels of {buf.dtype}, expected {N} x {C} of {dt}")
+        structs.append(_pack_view(buf.data_ptr(), H, W, halo, total, v.ch_offset))
     for name, t in vectors:
         if t.get_device() != dev:
             _require_cuda(t, f"{what}: {name}")
