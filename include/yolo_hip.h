@@ -420,8 +420,9 @@ size_t yolo_grad_norm_workspace_bytes(int n_blocks);
  * out like norms: min(1, max_norm / (norm + 1e-6)).  Sums are fp64, joined in the table's order. */
 int yolo_grad_norm(const yolo_grad_block* blocks, int n_blocks, const int* tensor_first, int n_tensors, float norm_type,
                    float max_norm, float* norms, float* coefs, void* workspace, size_t ws_bytes, void* stream);
-/* g *= coefs[0], or coefs[tensor of the run] */
-int yolo_grad_scale(const yolo_grad_block* blocks, int n_blocks, const float* coefs, int per_tensor, void* stream);
+/* yolo_grad_norm, then g *= norms' factor: coefs[0], or coefs[tensor of the run] */
+int yolo_grad_clip(const yolo_grad_block* blocks, int n_blocks, const int* tensor_first, int n_tensors, float norm_type,
+                   float max_norm, float* norms, float* coefs, void* workspace, size_t ws_bytes, void* stream);
 /* g = min(max(g, -value), value), a NaN stays */
 int yolo_grad_clamp(const yolo_grad_block* blocks, int n_blocks, float value, void* stream);
 

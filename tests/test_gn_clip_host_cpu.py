@@ -71,8 +71,9 @@ def test_grad_refusals():
                        ((p, -1, None, 0, 2.0, 1.0, p, p, p, 8), "blocks"), ((p, 1, p, 0, 2.0, 1.0, p, p, p, 8), "tensors"),
                        ((p, 1, None, 0, 3.0, 1.0, p, p, p, 8), "norm type"), ((p, 1, None, 0, -inf, 1.0, p, p, p, 8), "norm type"),
                        ((p, 1, None, 0, 2.0, -1.0, p, p, p, 8), "max_norm"), ((p, 2, None, 0, inf, 1.0, p, p, p, 8), "workspace")):
-        assert L.yolo_grad_norm(*args, None) < 0 and says in L.yolo_last_error().decode(), says
-    assert L.yolo_grad_scale(p, 1, None, 0, None) < 0 and L.yolo_grad_clamp(p, 1, -1.0, None) < 0
+        for call in (L.yolo_grad_norm, L.yolo_grad_clip):
+            assert call(*args, None) < 0 and says in L.yolo_last_error().decode(), says
+    assert L.yolo_grad_clip(p, 1, None, 0, 2.0, 1.0, p, None, p, 8, None) < 0 and L.yolo_grad_clamp(p, 1, -1.0, None) < 0
     assert L.yolo_grad_clamp(p, 1, float("nan"), None) < 0
     step = lambda w, n, coefs, v: L.yolo_sgd_step_clipped(w, p, p, p, n, 0.1, 0.0, 0.1, 0.0, 0.9, coefs, 0, v, None)  # noqa: E731
     assert step(None, 1, p, 0.0) < 0 and step(p, 0, p, 0.0) < 0 and step(p, 1, None, -1.0) < 0 and step(p + 4, 1, p, 0.0) < 0

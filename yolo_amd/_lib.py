@@ -113,7 +113,8 @@ SIGNATURES = {
     "yolo_grad_norm_workspace_bytes": (c_size_t, [c_int]),
     "yolo_grad_norm": (c_int, [c_void_p, c_int, c_void_p, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p, c_size_t,
                                c_void_p]),
-    "yolo_grad_scale": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p]),
+    "yolo_grad_clip": (c_int, [c_void_p, c_int, c_void_p, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p, c_size_t,
+                               c_void_p]),
     "yolo_grad_clamp": (c_int, [c_void_p, c_int, c_float, c_void_p]),
     "yolo_sgd_step_clipped": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_float, c_float, c_float,
                                       c_float, c_void_p, c_int, c_float, c_void_p]),

@@ -987,7 +987,7 @@ def _dense_run(t: torch.Tensor) -> bool:
 
 def grad_table(tensors: Sequence[torch.Tensor]) -> GradTable:
     """Table of ``tensors`` (float32 or bfloat16, each one run of memory in some dimension order, none twice) for grad_norm,
-    grad_scale and grad_clamp.  Built on the host and copied once: build it outside graph capture."""
+    grad_clip and grad_clamp.  Built on the host and copied once: build it outside graph capture."""
     tensors = list(tensors)
     if not tensors:
         raise ValueError("grad_table: no tensors")
@@ -1032,31 +1032,32 @@ def _check_norms(t: Optional[torch.Tensor], n: int, what: str, dev: int) -> None
         raise ValueError(f"{what}: expected a contiguous float32 tensor of {n}")
 
 
+def _grad_norm_args(what: str, table: GradTable, norms, workspace, norm_type, per_tensor, max_norm, coefs):
+    n, dev = len(table.tensors) if per_tensor else 1, table.blocks.get_device()
+    if dev != torch.cuda.current_device():
+        _require_cuda(table.blocks, what)
+    _check_norms(norms, n, f"{what}: norms", dev)
+    _check_norms(coefs, n, f"{what}: coefs", dev)
+    if workspace.get_device() != dev:
+        _require_cuda(workspace, f"{what}: workspace")
+    return (table.blocks.data_ptr(), table.n_blocks, table.first.data_ptr() if per_tensor else None, n, norm_type, max_norm,
+            norms.data_ptr(), None if coefs is None else coefs.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _stream_of(dev))
+
+
 def grad_norm(table: GradTable, norms: torch.Tensor, workspace: torch.Tensor, *, norm_type: float = 2.0,
               per_tensor: bool = False, max_norm: float = 0.0, coefs: Optional[torch.Tensor] = None) -> None:
     """norms [1] <- the norm (1, 2 or inf) of all the table's tensors together, or [n_tensors] <- of each; coefs, of the same
     length, <- min(1, max_norm / (norm + 1e-6)).  Nothing is read back to the host."""
-    n, dev = len(table.tensors) if per_tensor else 1, table.blocks.get_device()
-    if dev != torch.cuda.current_device():
-        _require_cuda(table.blocks, "grad_norm")
-    _check_norms(norms, n, "grad_norm: norms", dev)
-    _check_norms(coefs, n, "grad_norm: coefs", dev)
-    if workspace.get_device() != dev:
-        _require_cuda(workspace, "grad_norm: workspace")
-    check(lib().yolo_grad_norm(table.blocks.data_ptr(), table.n_blocks, table.first.data_ptr() if per_tensor else None,
-                               n, norm_type, max_norm, norms.data_ptr(), None if coefs is None else coefs.data_ptr(),
-                               workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream_of(dev)),
+    check(lib().yolo_grad_norm(*_grad_norm_args("grad_norm", table, norms, workspace, norm_type, per_tensor, max_norm, coefs)),
           "yolo_grad_norm")
 
 
-def grad_scale(table: GradTable, coefs: torch.Tensor, *, per_tensor: bool = False) -> None:
-    """Multiply the table's tensors by coefs [1], or each by its own of coefs [n_tensors], in place."""
-    dev = table.blocks.get_device()
-    if dev != torch.cuda.current_device():
-        _require_cuda(table.blocks, "grad_scale")
-    _check_norms(coefs, len(table.tensors) if per_tensor else 1, "grad_scale: coefs", dev)
-    check(lib().yolo_grad_scale(table.blocks.data_ptr(), table.n_blocks, coefs.data_ptr(), int(per_tensor), _stream_of(dev)),
-          "yolo_grad_scale")
+def grad_clip(table: GradTable, norms: torch.Tensor, coefs: torch.Tensor, workspace: torch.Tensor, *, max_norm: float,
+              norm_type: float = 2.0, per_tensor: bool = False) -> None:
+    """grad_norm, and the table's tensors multiplied by coefs [1], or each by its own of coefs [n_tensors], in place."""
+    check(lib().yolo_grad_clip(*_grad_norm_args("grad_clip", table, norms, workspace, norm_type, per_tensor, max_norm, coefs)),
+          "yolo_grad_clip")
 
 
 def grad_clamp(table: GradTable, value: float) -> None:

@@ -49,9 +49,6 @@ class GradientClipper:
     def measure(self) -> Optional[torch.Tensor]:
         """The norms the clipping goes by ([1] or [n_tensors], overwritten by the next call; ``coefs`` has the factors);
         None for "value".  The gradients are only read."""
-        return self._measure()
-
-    def _measure(self) -> Optional[torch.Tensor]:
         if self.clip_type == "value":
             return None
         ops.grad_norm(self.table, self.norms, self._ws, norm_type=self.norm_type, per_tensor=self.per_tensor,
@@ -60,13 +57,13 @@ class GradientClipper:
 
     @ops.on_own_device
     def clip_(self) -> Optional[torch.Tensor]:
-        """measure(), then the gradients clipped in place."""
-        norms = self._measure()
+        """measure(), and the gradients clipped in place."""
         if self.clip_type == "value":
             ops.grad_clamp(self.table, self.clip_value)
-        else:
-            ops.grad_scale(self.table, self.coefs, per_tensor=self.per_tensor)
-        return norms
+            return None
+        ops.grad_clip(self.table, self.norms, self.coefs, self._ws, max_norm=self.clip_value, norm_type=self.norm_type,
+                      per_tensor=self.per_tensor)
+        return self.norms
 
 
 def _grads(parameters) -> List[torch.Tensor]:
