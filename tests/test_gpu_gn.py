@@ -120,6 +120,25 @@ def test_forward(cuda, shape, dtype, act, slope):
         _check_forward(x, res, gamma, beta, G, act, slope, yv.interior(), stats)
 
 
+# every CU has a slab that its registers do not hold: the rest in LDS, or read again too; far means as well
+@pytest.mark.parametrize("dtype,shape,act,far", [(torch.bfloat16, (256, 59, 51, 64, 32), "leaky", 0.0),
+                                                 (torch.float32, (256, 59, 51, 32, 8), "silu", 100.0),
+                                                 (torch.bfloat16, (256, 66, 61, 64, 4), "silu", 0.0)], ids=ids)
+def test_forward_of_tall_slabs(cuda, dtype, shape, act, far):
+    from yolo_amd import ops
+    x, r, _, gamma, beta = _inputs(shape, dtype)
+    N, H, W, C, G = shape
+    x = x + far
+    for res in (None, r):
+        _, yv, stats, ws = _forward(cuda, x, res, gamma, beta, G, act, 0.1, halo=(1, 0, 2))
+        _check_forward(x, res, gamma, beta, G, act, 0.1, yv.interior(), stats)
+    for over_x in (False, True):   # in place: the same bits
+        xv, rv = _view(x, cuda, 1), _view(r, cuda, 1)
+        out, again = (xv if over_x else rv), torch.empty_like(stats)
+        ops.gn_act_fwd(xv, gamma.to(cuda), beta.to(cuda), out, again, ws, groups=G, act=act, slope=0.1, residual=rv)
+        assert torch.equal(out.interior(), yv.interior()) and torch.equal(again, stats)
+
+
 def _ref_backward(x, dy, gamma, beta, mean, rs, G, act, slope):
     """The formulas at given statistics, in 64 bits; (dx, dgamma, dbeta) and their tolerances' sizes."""
     N, H, W, C = x.shape

@@ -662,9 +662,9 @@ struct GnWalk {
 #pragma unroll
         for (int k = 0; k < K; ++k) at0[k] = c.at[k];
     }
-    template <int ST>
+    template <int ST, bool ALL>
     __device__ __forceinline__ u32x4 load(int k, int i, const GnSeat& s, const char* base) const {
-        return gn_load<ST>(base, i < s.count ? c.at[k] : at0[k]);
+        return gn_load<ST>(base, ALL || i < s.count ? c.at[k] : at0[k]);
     }
 };
 // ... and zeros there
@@ -694,18 +694,19 @@ __device__ __forceinline__ GnCursor<K> gn_again(const GnParams& p, const GnSeat&
 }
 
 // The sum over a wave's pixel lanes, valid in those of pixel lane 0.
-__device__ __forceinline__ float gn_over_pixels(float v, const GnParams& p, int pl, int top) {
+template <typename T>
+__device__ __forceinline__ T gn_over_pixels(T v, const GnParams& p, int pl, int top) {
     for (int o = top; o; o >>= 1) {
-        const float w = __shfl_down(v, o * p.VS);
-        v += pl + o < p.PL ? w : 0.f;
+        const T w = __shfl_down(v, o * p.VS);
+        v += pl + o < p.PL ? w : T(0);
     }
     return v;
 }
 
 // part[wave][cell] <- sums of the slab's cells (fold channels each) over the wave's pixels; then the group sums, handed to
 // done(group in the slab, sum, lane) in 16 lanes each.
-template <int V, typename F>
-__device__ __forceinline__ void gn_group_sums(float (&s)[V], float (*part)[GN_SLAB], const GnParams& p, const GnSeat& t, int groups,
+template <int V, typename T, typename F>
+__device__ __forceinline__ void gn_group_sums(T (&s)[V], T (*part)[GN_SLAB], const GnParams& p, const GnSeat& t, int groups,
                                               int top, F done) {
     if (p.fold >= 2)
 #pragma unroll
@@ -718,7 +719,7 @@ __device__ __forceinline__ void gn_group_sums(float (&s)[V], float (*part)[GN_SL
 #pragma unroll
     for (int e = 0; e < V; ++e)
         if ((e & (p.fold - 1)) == 0) {
-            const float v = gn_over_pixels(s[e], p, t.pl, top);
+            const T v = gn_over_pixels(s[e], p, t.pl, top);
             if (t.pl == 0 && t.on) part[t.wave][(t.cs + e) / p.fold] = v;
         }
     __syncthreads();
@@ -743,10 +744,19 @@ __device__ __forceinline__ int gn_top(int pl) {  // the first distance of a tree
     return o >> 1;
 }
 
-template <typename E, int ACT, int NV>
+//
+// TALL: slabs that do not fit.  A thread's first NV vectors are in registers, the next GN_KEPT_FWD in LDS, and what is left is read
+// again; those beyond NV are summed first, as in gn_sums_kernel (pivots; fp64 sums of values and squares), the others by the
+// definition.  64 x 60 x 60 x 256 bf16 with a residual: 75 us, with 64 B whole 100; without one 50 and 63.  Twelve vectors in
+// registers leave room for the residual's (14: 80 us, 16: 82 us; without one 50 and 49).
+constexpr int GN_KEPT_FWD = 8;
+template <typename E, int ACT, int NV, bool TALL = false>
 __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
-    __shared__ float part[GN_WAVES][GN_SLAB];
+    __shared__ double parts[TALL ? GN_WAVES : GN_WAVES / 2][GN_SLAB];
+    __shared__ u32x4 kept[TALL ? GN_KEPT_FWD : 1][TALL ? 1024 : 1];
+    __shared__ double others[2][TALL ? GN_SLAB : 1];  // by group: the sums of the values and squares that are not in registers
+    float (*part)[GN_SLAB] = (float (*)[GN_SLAB])parts;
     __shared__ __attribute__((aligned(16))) float mean_of[GN_SLAB], scale_of[GN_SLAB], shift_of[GN_SLAB];  // by channel
     __shared__ double off_of[GN_SLAB];  // by group: the mean minus its fp32 value
     const GnSeat t = gn_seat<E>(p);
@@ -756,29 +766,73 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
     const int mine = min((int)threadIdx.x, width - 1);  // width <= GN_SLAB <= threads; these two loads come back first
     const float gamma = p.gamma[c0 + mine], beta = p.beta[c0 + mine];
     const char* x = p.x.p + n * p.x.img;
+    const int more = TALL ? max(t.count - NV, 0) : 0;
+    if constexpr (TALL) {  // sums of differences from the thread's first value, as gn_sums_kernel
+        float k[V], s[V], q[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) k[e] = s[e] = q[e] = 0.f;
+        if (more) {
+            GnCursor<1> c(t.first + NV * t.step, t.step, p.W, cb, {&p.x});
+            const u32x4 r0 = gn_load(x, c.at[0]);
+            c.next();
+            kept[0][threadIdx.x] = r0;
+            GnVec<E>::unpack(r0, k);
+            int i = 1;
+            gn_pipelined<4, 1>(
+                more - 1,
+                [&](u32x4* r) {
+                    r[0] = gn_load(x, c.at[0]);
+                    c.next();
+                },
+                [&](const u32x4* r) {
+                    if (i < GN_KEPT_FWD) kept[i][threadIdx.x] = r[0];
+                    ++i;
+                    float f[V];
+                    GnVec<E>::unpack(r[0], f);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const float d = f[e] - k[e];
+                        s[e] += d;
+                        q[e] = fmaf(d, d, q[e]);
+                    }
+                });
+        }
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            double m[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const double K = k[e], sd = s[e];
+                m[e] = which == 0 ? more * K + sd : (double)q[e] + K * (2.0 * sd + more * K);
+            }
+            gn_group_sums<V>(m, parts, p, t, groups, top, [&](int g, double sum, int sub) {
+                if (sub == 0) others[which][g] = sum;
+            });
+        }
+    }
     u32x4 v[NV];
     gn_with_stream(p.stream, [&](auto st) {
         GnWalk<1> walk(p, t, cb, {&p.x});
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            v[i] = walk.template load<decltype(st)::value>(0, i, t, x);
+            v[i] = walk.template load<decltype(st)::value, TALL>(0, i, t, x);
             walk.c.next();
         }
     });
-    gn_blank<NV>(v, t);
+    if constexpr (!TALL) gn_blank<NV>(v, t);
     float s[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) s[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-        if (i < t.most) {
+        if (TALL || i < t.most) {
             float f[V];
             GnVec<E>::unpack(v[i], f);
 #pragma unroll
             for (int e = 0; e < V; ++e) s[e] += f[e];
         }
     gn_group_sums<V>(s, part, p, t, groups, top, [&](int g, double sum, int sub) {
-        const double mean = sum * p.inv_count;
+        const double mean = (TALL ? sum + others[0][g] : sum) * p.inv_count;
         for (int i = sub; i < p.Cg; i += 16) mean_of[g * p.Cg + i] = (float)mean;
         if (sub == 0) {
             off_of[g] = mean - (double)(float)mean;
@@ -794,7 +848,7 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
         for (int e = 0; e < 4; ++e) mean[e] = mean_of[t.cs + 4 * h + e];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (i < t.full || i < t.count) {
+            if (TALL || i < t.full || i < t.count) {
                 float f[4];
                 gn_part<E, 4>(v[i], h, f);
 #pragma unroll
@@ -807,6 +861,10 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
         for (int e = 0; e < 4; ++e) s[4 * h + e] = q[e];
     }
     gn_group_sums<V>(s, part, p, t, groups, top, [&](int g, double sum, int sub) {
+        if constexpr (TALL) {
+            const double m = mean_of[g * p.Cg], count = (double)(p.HW - NV * t.step) * p.Cg;
+            sum += others[1][g] + m * (m * count - 2.0 * others[0][g]);
+        }
         const double off = off_of[g], var = sum * p.inv_count - off * off;
         const float r = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps));
         for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) scale_of[i] = r;
@@ -837,14 +895,14 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
     constants(t.cs);
     gn_with_stream(p.stream, [&](auto st) {
         constexpr int ST = decltype(st)::value;
-        auto put = [&](int i, const u32x4* r, unsigned to) {
+        auto put = [&](const u32x4& raw, const u32x4* r, unsigned to) {
             if constexpr (NV > 16) {  // no registers to keep them: from LDS for each vector
                 int cs = t.cs;
                 asm volatile("" : "+v"(cs));
                 constants(cs);
             }
             float f[V];
-            GnVec<E>::unpack(v[i], f);
+            GnVec<E>::unpack(raw, f);
 #pragma unroll
             for (int e = 0; e < V; ++e) f[e] = gn_act<ACT>(fmaf(SHIFT ? f[e] : f[e] - mean[e], scale[e], shift[e]), p.slope);
             if (r) {
@@ -863,25 +921,74 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
             u32x4 r[AHEAD];
 #pragma unroll
             for (int i = 0; i < AHEAD && i < NV; ++i) {
-                r[i] = ahead.template load<ST>(0, i, t, res);
+                r[i] = ahead.template load<ST, TALL>(0, i, t, res);
                 ahead.c.next();
             }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const u32x4 now = r[i % AHEAD];
                 if (i + AHEAD < NV) {
-                    r[i % AHEAD] = ahead.template load<ST>(0, i + AHEAD, t, res);
+                    r[i % AHEAD] = ahead.template load<ST, TALL>(0, i + AHEAD, t, res);
                     ahead.c.next();
                 }
-                if (i < t.count) put(i, &now, c.at[0]);
+                if (TALL || i < t.count) put(v[i], &now, c.at[0]);
                 c.next();
             }
         } else {
             GnCursor<1> c = gn_again<1>(p, t, cb, {&p.y});
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                if (i < t.count) put(i, nullptr, c.at[0]);
+                if (TALL || i < t.count) put(v[i], nullptr, c.at[0]);
                 c.next();
+            }
+        }
+        if constexpr (TALL) {
+            int from = t.first + NV * t.step, left = max(t.count - NV, 0);
+            asm volatile("" : "+v"(from), "+v"(left)::"memory");  // not worked out ahead: the registers are full until here
+            const int there = min(left, GN_KEPT_FWD);
+            GnCursor<1> cy(from, t.step, p.W, cb, {&p.y});
+            GnCursor<1> cx(from + there * t.step, t.step, p.W, cb, {&p.x});
+            if (res) {
+                GnCursor<1> cr(from, t.step, p.W, cb, {&p.r});
+                int i = 0;
+                gn_pipelined<2, 1>(
+                    there,
+                    [&](u32x4* r) {
+                        r[0] = gn_load<ST>(res, cr.at[0]);
+                        cr.next();
+                    },
+                    [&](const u32x4* r) {
+                        put(kept[i][threadIdx.x], r, cy.at[0]);
+                        cy.next();
+                        ++i;
+                    });
+                gn_pipelined<2, 2>(
+                    left - there,
+                    [&](u32x4* r) {
+                        r[0] = gn_load<ST>(x, cx.at[0]);
+                        r[1] = gn_load<ST>(res, cr.at[0]);
+                        cx.next();
+                        cr.next();
+                    },
+                    [&](const u32x4* r) {
+                        put(r[0], r + 1, cy.at[0]);
+                        cy.next();
+                    });
+            } else {
+                for (int i = 0; i < there; ++i) {
+                    put(kept[i][threadIdx.x], nullptr, cy.at[0]);
+                    cy.next();
+                }
+                gn_pipelined<2, 1>(
+                    left - there,
+                    [&](u32x4* r) {
+                        r[0] = gn_load<ST>(x, cx.at[0]);
+                        cx.next();
+                    },
+                    [&](const u32x4* r) {
+                        put(r[0], nullptr, cy.at[0]);
+                        cy.next();
+                    });
             }
         }
     });
@@ -960,8 +1067,8 @@ __global__ void __launch_bounds__(1024) gn_whole_bwd_kernel(const GnParams p) {
         GnWalk<2> walk(p, t, cb, {&p.x, &p.dy});
 #pragma unroll
         for (int i = 0; i < NV; ++i) {  // in turn: the first pairs are used while the last ones are on their way
-            x[i] = walk.template load<decltype(st)::value>(0, i, t, xp);
-            d[i] = walk.template load<decltype(st)::value>(1, i, t, dp);
+            x[i] = walk.template load<decltype(st)::value, false>(0, i, t, xp);
+            d[i] = walk.template load<decltype(st)::value, false>(1, i, t, dp);
             walk.c.next();
         }
     });
@@ -1171,11 +1278,13 @@ static void gn_split(GnParams& p, int es) {
 //   64 B so that it fits, no less                64 x 104 x 104 x 128 forward 102 with 32 B, in chunks 97; one image 33 and 18
 // Forward a thread takes up to 11 vectors before the workgroup gets more waves (64 x 26 x 26 x 512: 17.8 us with 8 waves of 11, 23.3
 // with 16 of 6); backward it has two tensors' vectors, and spills above 8.  Taller slabs are then held in part, at 128 B a pixel,
-// where the CUs, one slab each, are busy (backward):
-//   half of the CUs and more, up to 32 vectors   64 x 52 x 52 x 256 68.0, in chunks 83;  32 images 44 and 52;  16 images 37 and 32
+// where the CUs, one slab each, are busy:
+//   backward, half of the CUs and more, to 32    64 x 52 x 52 x 256 68.0, in chunks 83;  32 images 44 and 52;  16 images 37 and 32
 //                                                64 x 40 x 40 x 256 41, with 64 B whole 64
-//   all of them, up to 64 vectors                64 x 76 x 76 x 256 150, in chunks 161;  64 x 76 x 76 x 128 (128 slabs) 91 and 87
-//   several slabs each, the last round not empty 96 x 52 x 52 x 256 (384 slabs) 110, in chunks 117;  80 images (320) 104 and 99
+//   all of them, up to 64 vectors                64 x 76 x 76 x 256 backward 150, in chunks 161;  64 x 76 x 76 x 128 (128 slabs) 91 and 87
+//                                                64 x 76 x 76 x 256 forward 82, in chunks 103;  64 x 88 x 88 x 256 122 and 135
+//                                                32 x 60 x 60 x 256 forward (128 slabs) 32, with 64 B whole 31
+//   several slabs each, the last round not empty 96 x 52 x 52 x 256 backward (384 slabs) 110, in chunks 117;  80 images (320) 104 and 99
 struct GnWhole {
     int VS, waves, NV;
     bool tall;
@@ -1195,8 +1304,8 @@ static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out
     if (blocks(VS) < 512 || nv(VS, GN_WAVES) > nv_most) VS = fit(8);
     const long long there = blocks(VS), rounds = (there + 255) / 256;  // a tall slab takes a CU of its own
     const int tall = nv(VS, GN_WAVES);
-    const bool busy = there <= 256 ? there >= (tall <= 32 ? 128 : 256) : there * 10 >= rounds * 256 * 7;
-    if (backward && tall > nv_most && tall <= 64 && (VS % 8 == 0 || VS == vecs) && busy) {
+    const bool busy = there <= 256 ? there >= (backward && tall <= 32 ? 128 : 256) : there * 10 >= rounds * 256 * 7;
+    if (tall > nv_most && tall <= 64 && (VS % 8 == 0 || VS == vecs) && busy) {
         *out = GnWhole{VS, GN_WAVES, tall, true};
         return true;
     }
@@ -1323,6 +1432,9 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
         p.slabs = (p.C * es / 16 + w.VS - 1) / w.VS;
         p.stream = p.stream && w.VS % 8 == 0;  // whole cache lines only
         const dim3 grid((unsigned)(p.slabs * N));
+        if (w.tall)
+            GN_LAUNCH(grid, dim3(1024), gn_whole_kernel, 12, true);
+        else
         GN_WHOLE_CASE(gn_whole_kernel, 1)
         GN_WHOLE_CASE(gn_whole_kernel, 2)
         GN_WHOLE_CASE(gn_whole_kernel, 4)
