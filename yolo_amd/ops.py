@@ -991,32 +991,37 @@ def grad_table(tensors: Sequence[torch.Tensor]) -> GradTable:
     tensors = list(tensors)
     if not tensors:
         raise ValueError("grad_table: no tensors")
+    dev = tensors[0].get_device()
+    _require_cuda(tensors[0], "grad_table")
+    ptrs, counts, codes, sizes = [], [], [], []
     for t in tensors:
-        _require_cuda(t, "grad_table")
-        dtype_code(t.dtype)
-        if t.numel() and not _dense_run(t):
+        if t.get_device() != dev:
+            _require_cuda(t, "grad_table")
+        n = t.numel()
+        if n and not t.is_contiguous() and not _dense_run(t):
             raise ValueError(f"grad_table: a tensor {tuple(t.shape)} with strides {tuple(t.stride())} is not one run of memory")
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel())
-    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        ptrs.append(t.data_ptr())
+        counts.append(n)
+        codes.append(dtype_code(t.dtype))
+        sizes.append(t.element_size())
+    ptrs, counts, codes, sizes = np.array(ptrs, np.uint64), np.array(counts, np.int64), np.array(codes), np.array(sizes, np.int64)
+    lo = np.sort(ptrs[counts > 0])
+    hi = np.sort((ptrs + (counts * sizes).astype(np.uint64))[counts > 0])
+    if (lo[1:] < hi[:-1]).any():   # sorted by their begins and by their ends, runs of memory that do not meet are in one order
         raise ValueError("grad_table: two tensors share memory (a shared gradient is listed once)")
     # runs of a workgroup: 16384 elements, down to 4096 where the whole set would not give each CU eight
-    total = sum(t.numel() for t in tensors)
-    run = max(4096, min(16384, total // 2048 // 1024 * 1024))
-    counts = np.array([t.numel() for t in tensors], np.int64)
+    run = max(4096, min(16384, int(counts.sum()) // 2048 // 1024 * 1024))
     runs = -(-counts // run)
-    first = np.concatenate([[0], np.cumsum(runs)])
+    first = np.concatenate([[0], np.cumsum(runs)]).astype(np.int32)
     owner = np.repeat(np.arange(len(tensors)), runs)
     begin = (np.arange(first[-1]) - first[owner]) * run     # a run's first element in its tensor
-    sizes = np.array([t.element_size() for t in tensors], np.int64)
-    blocks = np.zeros(max(1, len(owner)), np.dtype(GradBlock))
-    rows = blocks[:len(owner)]
-    rows["ptr"] = np.array([t.data_ptr() for t in tensors], np.uint64)[owner] + (begin * sizes[owner]).astype(np.uint64)
+    rows = np.zeros(len(owner), np.dtype(GradBlock))
+    rows["ptr"] = ptrs[owner] + (begin * sizes[owner]).astype(np.uint64)
     rows["count"] = np.minimum(run, counts[owner] - begin)
     rows["tensor"] = owner
-    rows["dtype"] = np.array([dtype_code(t.dtype) for t in tensors])[owner]
-    dev = tensors[0].device
-    return GradTable(torch.from_numpy(blocks.view(np.uint8)).to(dev), len(rows),
-                     torch.from_numpy(first.astype(np.int32)).to(dev), tensors)
+    rows["dtype"] = codes[owner]
+    both = torch.from_numpy(np.concatenate([rows.view(np.uint8), first.view(np.uint8)])).to(tensors[0].device)
+    return GradTable(both[:rows.nbytes], len(rows), both[rows.nbytes:].view(torch.int32), tensors)
 
 
 def grad_norm_workspace_bytes(table: GradTable) -> int:

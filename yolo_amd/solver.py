@@ -39,7 +39,7 @@ class GradientClipper:
         self.norms = self.coefs = self._ws = None
         if clip_type != "value" and grads:   # filled by the time the table's synchronous copy is done: any stream may come next
             n = len(grads) if self.per_tensor else 1
-            self.norms, self.coefs = torch.zeros(n, device=grads[0].device), torch.ones(n, device=grads[0].device)
+            self.norms, self.coefs = torch.ones(2, n, device=grads[0].device)
         self.table = ops.grad_table(grads)
         self.device = self.table.blocks.device
         if self.norms is not None:
