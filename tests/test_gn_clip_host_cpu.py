@@ -117,6 +117,10 @@ def test_clip_settings():
                          "SOLVER.CLIP_GRADIENTS.CLIP_VALUE", 10.0])
     opt = solver.build_optimizer(cfg, model)
     assert opt._clip == ("full_model", 10.0, 2.0)
+    for word in ("inf", ".inf", float("inf")):
+        c = cfg.clone()
+        c.merge_from_list(["SOLVER.CLIP_GRADIENTS.NORM_TYPE", word])
+        assert solver.build_optimizer(c, model)._clip == ("full_model", 10.0, float("inf"))
     opt.step()                     # no gradients: nothing to clip
     with pytest.raises(RuntimeError, match="closure"):
         opt.step(lambda: 0.0)

@@ -79,6 +79,8 @@ class CfgNode(dict):
             return list(new)
         if isinstance(old, float) and isinstance(new, int) and not isinstance(new, bool):
             return float(new)
+        if isinstance(old, float) and new in ("inf", ".inf"):   # no Python literal, and YAML's only in files
+            return float("inf")
         raise ValueError(f"Type mismatch ({type(old)} vs. {type(new)}) for config key: {key}")
 
     def _merge(self, other: dict, path: List[str]) -> None:
