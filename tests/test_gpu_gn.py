@@ -22,7 +22,8 @@ OUT = {torch.float32: U, torch.bfloat16: 2.0 ** -8}
 # not full, more chunks than one, the network's own stages
 SHAPES = [(1, 1, 1, 8, 8), (2, 1, 1, 8, 1), (3, 2, 3, 24, 8), (2, 5, 7, 96, 32), (1, 13, 13, 1024, 32), (2, 13, 13, 512, 32),
           (1, 3, 5, 1024, 1), (2, 4, 3, 2056, 8), (5, 26, 25, 256, 32), (1, 52, 52, 128, 32), (2, 61, 47, 64, 32),
-          (1, 104, 90, 32, 32), (70, 6, 5, 384, 32), (3, 17, 1, 40, 5), (2, 1, 300, 72, 6), (1, 208, 200, 16, 2)]
+          (1, 104, 90, 32, 32), (70, 6, 5, 384, 32), (3, 17, 1, 40, 5), (2, 1, 300, 72, 6), (1, 208, 200, 16, 2),
+          (1, 208, 200, 64, 32), (64, 96, 50, 16, 2), (3, 50, 45, 96, 4), (8, 52, 40, 256, 32)]
 ids = lambda s: "x".join(map(str, s)) if isinstance(s, tuple) else str(s).replace("torch.", "")  # noqa: E731
 
 

@@ -349,6 +349,10 @@ __global__ void __launch_bounds__(GN_THREADS, 5) gn_sums_kernel(const GnParams p
     }
 }
 
+__device__ __forceinline__ float gn_rstd(const GnParams& p, double var) {
+    return (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps));
+}
+
 // The chunks' sums of the groups of about 64 channels of one image, in fp64 and in the chunks' order: lanes are channels, the
 // sixteen waves take the chunks in turn.  Forward: mean and r of a group.  Backward: the image's sums of each channel, and the
 // group's two terms from gamma times them.  Latency-bound, 4 to 5 us.
@@ -406,30 +410,89 @@ __global__ void __launch_bounds__(GN_JOIN * 64) gn_join_kernel(const GnParams p)
     } else {
         const double mean = A * p.inv_count, var = B * p.inv_count - mean * mean;
         p.stats[g] = (float)mean;
-        p.stats[p.N * p.groups + g] = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps));
+        p.stats[p.N * p.groups + g] = gn_rstd(p, var);
     }
 }
 
+// The same for the `width` channels of a slab (whole groups) from c0 on, by a workgroup that goes on with them: the group sums of its
+// groups, handed to done(group in the slab, sum, sum, lane) in 16 lanes each.
+template <bool BWD, typename F>
+__device__ __forceinline__ void gn_join_slab(const GnParams& p, int n, int c0, int width, double (*red)[GN_THREADS], F done) {
+    typedef typename std::conditional<BWD, float, double>::type P;
+    const int rows = GN_THREADS / width, row = threadIdx.x / width, col = threadIdx.x - row * width;
+    const P* part = (const P*)p.partial + (long long)n * p.chunks * 2 * p.C + c0 + col;
+    double a = 0.0, b = 0.0;
+    if (row < rows)
+#pragma unroll 8
+        for (int i = row; i < p.chunks; i += rows) {
+            a += (double)part[(long long)i * 2 * p.C];
+            b += (double)part[((long long)i * 2 + 1) * p.C];
+        }
+    red[0][threadIdx.x] = a;
+    red[1][threadIdx.x] = b;
+    __syncthreads();
+    if ((int)threadIdx.x < width) {
+        for (int r = 1; r < rows; ++r) {
+            a += red[0][r * width + threadIdx.x];
+            b += red[1][r * width + threadIdx.x];
+        }
+        const double gamma = BWD ? p.gamma[c0 + threadIdx.x] : 1.f;
+        red[0][threadIdx.x] = gamma * a;
+        red[1][threadIdx.x] = gamma * b;
+    }
+    __syncthreads();
+    const int sub = threadIdx.x & 15, groups = width / p.Cg;
+    for (int g0 = 0; g0 < groups; g0 += GN_THREADS / 16) {
+        const int g = g0 + (threadIdx.x >> 4);
+        double A = 0.0, B = 0.0;
+        if (g < groups)
+            for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) {
+                A += red[0][i];
+                B += red[1][i];
+            }
+        for (int o = 8; o; o >>= 1) {
+            A += __shfl_xor(A, o);
+            B += __shfl_xor(B, o);
+        }
+        if (g < groups) done(g, A, B, sub);
+    }
+    __syncthreads();
+}
 // ------------------------------------------------------------------------------------------------ forward, output
 // y = act((x - mean) * (gamma r) + beta) [+ residual], images and chunks in the reverse order of the sums: what was read last is
 // still in the cache in front of HBM.  64 x 208 x 208 x 64 bf16: 709 MB in 123 us, 5.8 TB/s.
-template <typename E, int ACT>
-__global__ void __launch_bounds__(GN_THREADS, 8) gn_apply_kernel(const GnParams p) {
+template <typename E, int ACT, bool JOIN = false>
+__global__ void __launch_bounds__(GN_THREADS, JOIN ? 6 : 8) gn_apply_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
+    __shared__ double red[2][JOIN ? GN_THREADS : 1];
+    __shared__ float of[2][JOIN ? GN_THREADS : 1];
     // fp32: (x - mean) * scale + beta; bf16: x * scale + (beta - mean * scale), whose rounding of mean * scale is far below the
     // output's
     constexpr bool SHIFT = sizeof(E) == 2;
     const GnLane l = gn_lane<E>(p);
     // the pass before this one walked forwards: its last chunks are the ones still in the caches
     const int n = p.N - 1 - blockIdx.z, chunk = p.chunks - 1 - blockIdx.x;
-    const int first = chunk * p.chunk, last = min(first + p.chunk, p.HW);
+    const int first = chunk * p.chunk, last = min(first + p.chunk, p.HW), c0 = blockIdx.y * p.VS * V;
+    if constexpr (JOIN)
+        gn_join_slab<false>(p, n, c0, min(p.VS * V, p.C - c0), (double (*)[GN_THREADS])red, [&](int g, double A, double B, int sub) {
+            const double m = A * p.inv_count;
+            const float mean = (float)m, r = gn_rstd(p, B * p.inv_count - m * m);
+            for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) {
+                of[0][i] = mean;
+                of[1][i] = r;
+            }
+            if (sub == 0 && chunk == 0) {
+                p.stats[n * p.groups + c0 / p.Cg + g] = mean;
+                p.stats[(p.N + n) * p.groups + c0 / p.Cg + g] = r;
+            }
+        });
     if (!l.on || first + l.pl >= last) return;
     float mean[V], scale[V], shift[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int g = (l.c + e) / p.Cg;
-        mean[e] = p.stats[n * p.groups + g];
-        scale[e] = p.gamma[l.c + e] * p.stats[(p.N + n) * p.groups + g];
+        mean[e] = JOIN ? of[0][l.c - c0 + e] : p.stats[n * p.groups + g];
+        scale[e] = p.gamma[l.c + e] * (JOIN ? of[1][l.c - c0 + e] : p.stats[(p.N + n) * p.groups + g]);
         shift[e] = SHIFT ? fmaf(-mean[e], scale[e], p.beta[l.c + e]) : p.beta[l.c + e];
     }
     const int cb = l.c * (int)sizeof(E);
@@ -531,12 +594,12 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_sums_kernel(const GnPara
 
 // dgamma, dbeta: the images' sums.  A workgroup has 32 of the 2 C columns (d sums, then d * xh sums), the i-th such set of them,
 // and eight rows at a time.
-__device__ __forceinline__ void gn_params(const GnParams& p, int set, double (*red)[32]) {
+__device__ __forceinline__ void gn_params(const GnParams& p, int set, double (*red)[32], const float* sums, int rows) {
     const int col = threadIdx.x & 31, row = threadIdx.x >> 5, i = set * 32 + col;
     double a = 0.0;
     if (i < 2 * p.C)
 #pragma unroll 8
-        for (int n = row; n < p.N; n += 8) a += (double)p.sums[(long long)n * 2 * p.C + i];
+        for (int n = row; n < rows; n += 8) a += (double)sums[(long long)n * 2 * p.C + i];
     red[row][col] = a;
     __syncthreads();
     if (row == 0 && i < 2 * p.C) {
@@ -550,20 +613,20 @@ __device__ __forceinline__ void gn_params(const GnParams& p, int set, double (*r
 }
 __global__ void __launch_bounds__(GN_THREADS) gn_bwd_params_kernel(const GnParams p) {
     __shared__ double red[8][32];
-    gn_params(p, blockIdx.x, red);
+    gn_params(p, blockIdx.x, red, p.sums, p.N);
 }
 
 // ------------------------------------------------------------------------------------------------ backward, output
 // dx = d * scale - (x - mean) * (r r B) - r A, four pixels at a time, images and chunks in the reverse order of the sums (64 x
 // 208 x 208 x 64 bf16: 1063 MB in 178 us, 6.0 TB/s).  The first plane of the grid sums dgamma and dbeta: a launch
 // of its own for them is 3 us.
-template <typename E, int ACT>
+template <typename E, int ACT, bool JOIN = false>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_apply_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
     __shared__ __attribute__((aligned(16))) float lds[4 * GN_THREADS * V];
     if (blockIdx.z == 0) {
         for (int set = blockIdx.y * p.chunks + blockIdx.x; set * 32 < 2 * p.C; set += p.chunks * gridDim.y)
-            gn_params(p, set, (double (*)[32])lds);
+            gn_params(p, set, (double (*)[32])lds, JOIN ? (const float*)p.partial : p.sums, JOIN ? p.N * p.chunks : p.N);
         return;
     }
     const GnLane l = gn_lane<E>(p);
@@ -571,15 +634,24 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_apply_kernel(const GnPar
     const int first = chunk * p.chunk, last = min(first + p.chunk, p.HW);
     const float* mine = lds + (l.c - blockIdx.y * S);
     gn_stage(lds, p, n, blockIdx.y * S, S);
+    float* terms = lds + 4 * GN_THREADS;  // JOIN: behind the constants of at most GN_THREADS channels; then the sums to join
+    if constexpr (JOIN)
+        gn_join_slab<true>(p, n, blockIdx.y * S, min(S, p.C - (int)blockIdx.y * S), (double (*)[GN_THREADS])(lds + 6 * GN_THREADS),
+                           [&](int g, double A, double B, int sub) {
+                               for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) {
+                                   terms[i] = (float)(A * p.inv_count);
+                                   terms[GN_THREADS + i] = (float)(B * p.inv_count);
+                               }
+                           });
     if (!l.on || first + l.pl >= last) return;
     const GnConst<V> k(mine, S);
     float k0[V], k1[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const int g = (l.c + e) / p.Cg;
+        const int g = (l.c + e) / p.Cg, c = l.c + e - blockIdx.y * S;
         const float r = p.stats[(p.N + n) * p.groups + g];
-        k0[e] = -r * p.terms[n * p.groups + g];
-        k1[e] = -r * r * p.terms[(p.N + n) * p.groups + g];
+        k0[e] = -r * (JOIN ? terms[c] : p.terms[n * p.groups + g]);
+        k1[e] = -r * r * (JOIN ? terms[GN_THREADS + c] : p.terms[(p.N + n) * p.groups + g]);
     }
     const float near = gn_near<V>(k.beta);
     const int cb = l.c * (int)sizeof(E);
@@ -866,7 +938,7 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
             sum += others[1][g] + m * (m * count - 2.0 * others[0][g]);
         }
         const double off = off_of[g], var = sum * p.inv_count - off * off;
-        const float r = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps));
+        const float r = gn_rstd(p, var);
         for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) scale_of[i] = r;
         if (sub == 0) p.stats[(p.N + n) * p.groups + g0 + g] = r;
     });
@@ -1253,6 +1325,12 @@ static int gn_check_shape(int N, int C, int groups, int act, float slope, int dt
     return YOLO_OK;
 }
 
+static int gn_unit(const GnParams& p, int V) {  // vectors of the smallest slab: whole groups, whole vectors
+    int unit = p.Cg;
+    while (unit % V) unit += p.Cg;
+    return unit / V;
+}
+
 // The split of an image over workgroups: pixel chunks so that about 2048 workgroups (8 per CU) are there, but no more than 256
 // chunks for that (what joins them reads them all), no fewer than 4 pixels to a thread, and no more than 128 (its fp32 sums).
 static void gn_split(GnParams& p, int es) {
@@ -1268,6 +1346,32 @@ static void gn_split(GnParams& p, int es) {
     if (chunk > 128ll * p.PL) chunk = 128ll * p.PL;
     p.chunk = (int)chunk;
     p.chunks = (int)((p.HW + chunk - 1) / chunk);
+}
+
+// The split for chunked passes without the joining launch: slabs of whole groups, about 128 B of a pixel, with so few chunks that a
+// workgroup of the second pass reads no more than 64 KB of sums.  For up to 32 MB of x, and workgroups that are short or many
+// (measured, bf16, us, with the joining launch and without):
+//   8 x 104 x 104 x 128 forward with a residual 30.6 and 26.9;  16 images (44 MB) 43.2 and 44.6;  8 x 80 x 80 x 128 backward 23.9 and 21.2
+//   1 x 104 x 104 x 64 (64 workgroups of 5 pixels a thread) forward 14.4 and 13.8;  1 x 208 x 208 x 64 (of 21 pixels) 18.5 and 22.6
+static bool gn_split_joined(GnParams& p, int es, bool backward) {
+    const int V = 16 / es, vecs = p.C / V, uv = gn_unit(p, V);
+    if (uv > 32) return false;
+    const int VS = uv > 8 ? uv : (vecs < 8 ? vecs : 8) / uv * uv, PL = GN_THREADS / VS, slabs = (vecs + VS - 1) / VS;
+    const int most = 65536 / (2 * VS * V * (backward ? 4 : 8));
+    long long want = 2048 / ((long long)p.N * slabs);
+    if (want < 1) want = 1;
+    if (want > most) want = most;
+    long long chunk = (p.HW + want - 1) / want;
+    if (chunk < 4ll * PL) chunk = 4ll * PL;
+    if (chunk > 128ll * PL) return false;
+    const long long chunks = (p.HW + chunk - 1) / chunk;
+    if ((long long)p.N * p.HW * p.C * es > (32ll << 20) || (chunk > 16ll * PL && p.N * slabs * chunks < 512)) return false;
+    p.VS = VS;
+    p.PL = PL;
+    p.chunk = (int)chunk;
+    p.chunks = (int)chunks;
+    p.stream = p.stream && (VS % 8 == 0 || VS == vecs);
+    return !backward || (long long)p.N * p.chunks <= 512;  // rows that dgamma and dbeta are summed over
 }
 
 // Whether (and how) workgroups can hold the slabs of an image.  The slab's width, in bytes of a pixel, decides how whole the cache
@@ -1291,9 +1395,7 @@ struct GnWhole {
 };
 static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out) {
     const int V = 16 / es, vecs = p.C / V;
-    int unit = p.Cg;  // smallest slab: whole groups, whole vectors
-    while (unit % V) unit += p.Cg;
-    const int uv = unit / V, most = GN_SLAB / V < vecs ? GN_SLAB / V : vecs;
+    const int uv = gn_unit(p, V), most = GN_SLAB / V < vecs ? GN_SLAB / V : vecs;
     if (uv > most) return false;
     const int nv_many = backward ? 6 : 11, nv_most = backward ? 8 : 22;
     auto fit = [&](int vs) { return vs < uv ? uv : (vs < most ? vs : most) / uv * uv; };  // whole units, about vs vectors
@@ -1319,6 +1421,20 @@ static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out
     out->waves = waves;
     out->NV = nv(VS, waves);
     return true;
+}
+
+// Where both are possible, the chunked passes without the joining launch have every CU at work on few images, and whole slabs x in
+// registers.  Measured (us, whole and chunked):
+//   forward   with a residual, 80 KB and more to each of less than 256 workgroups: bf16 1 x 52 x 52 x 256 17.2 and 13.2, 8 images 19.1
+//             and 18.4, 16 (256 workgroups) 26.1 and 27.7, 1 x 26 x 26 x 512 (28 KB) 7.3 and 10.9;  8 without a residual 15.0 and 17.5
+//   backward  bf16, less than 512 slabs of 128 B: 1 x 40 x 40 x 256 20.6 and 11.1, 24 x 13 x 13 x 1024 (384) 18.1 and 16.8, 32 (512) 19.5
+//             and 19.9;  16 MB and less: 16 x 26 x 26 x 512 20.0 and 18.3, 32 (22 MB) 27.2 and 29.2
+//             f32, less than 128: 4 x 26 x 26 x 512 (64) 13.2 and 12.9, 8 x 13 x 13 x 1024 (256) 11.8 and 13.1
+static bool gn_whole_first(const GnParams& p, int es, bool backward, const GnWhole& w) {
+    const int vecs = p.C * es / 16;
+    if (w.tall) return true;
+    if (!backward) return !p.r.p || w.waves * w.NV < 80 || (long long)p.N * ((vecs + w.VS - 1) / w.VS) >= 256;
+    return (long long)p.N * ((vecs + 7) / 8) >= (es == 2 ? 512 : 128) || (long long)p.N * p.HW * p.C * es > (16ll << 20);
 }
 
 static dim3 gn_join_grid(const GnParams& p) {
@@ -1386,11 +1502,17 @@ extern "C" size_t yolo_gn_workspace_bytes(int N, int H, int W, int C, int groups
     if (N <= 0 || H <= 0 || W <= 0 || C <= 0 || C % 8 || groups <= 0 || C % groups || (long long)H * W >= (1ll << 31)) return 0;
     GnParams p{};
     yolo_view v{nullptr, H, W, 0, C, 0};
-    gn_shape(p, &v, N, C, groups, (int)elem_size(dtype));
+    const int es = (int)elem_size(dtype);
+    gn_shape(p, &v, N, C, groups, es);
     // forward: the double sums; backward: the float sums, then the images' sums and the groups' terms
-    const size_t fwd = (size_t)N * p.chunks * 2 * C * sizeof(double);
-    const size_t bwd = ((size_t)N * p.chunks * 2 * C + (size_t)N * 2 * C + (size_t)2 * N * groups) * sizeof(float);
-    return fwd > bwd ? fwd : bwd;
+    auto sums = [&](const GnParams& q, size_t size) { return (size_t)N * q.chunks * 2 * C * size; };
+    size_t most = sums(p, sizeof(float)) + ((size_t)N * 2 * C + (size_t)2 * N * groups) * sizeof(float);
+    auto more = [&](size_t bytes) { most = bytes > most ? bytes : most; };
+    more(sums(p, sizeof(double)));
+    GnParams q = p;
+    if (gn_split_joined(q, es, false)) more(sums(q, sizeof(double)));
+    if (gn_split_joined(q, es, true)) more(sums(q, sizeof(float)));
+    return most;
 }
 
 extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const float* beta, const yolo_view* residual,
@@ -1425,7 +1547,9 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
     p.stream = gn_stream_rule(p, es, residual ? 3 : 2);
     hipStream_t st = (hipStream_t)stream;
     GnWhole w;
-    if (gn_whole_plan(p, es, false, &w)) {
+    GnParams q = p;
+    const bool joined = gn_split_joined(q, es, false);
+    if (gn_whole_plan(p, es, false, &w) && (!joined || gn_whole_first(p, es, false, w))) {
         p.VS = w.VS;
         p.PL = 64 / w.VS;
         p.fold = gn_fold(p.Cg, 16 / es);
@@ -1446,13 +1570,18 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
         YOLO_CHECK_HIP(hipGetLastError());
         return YOLO_OK;
     }
+    if (joined) p = q;
     const dim3 grid = gn_grid(p, es);
     if (dtype == YOLO_BF16)
         hipLaunchKernelGGL((gn_sums_kernel<unsigned short>), grid, dim3(GN_THREADS), 0, st, p);
     else
         hipLaunchKernelGGL((gn_sums_kernel<float>), grid, dim3(GN_THREADS), 0, st, p);
-    hipLaunchKernelGGL(gn_join_kernel<false>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
-    GN_LAUNCH(grid, dim3(GN_THREADS), gn_apply_kernel);
+    if (joined) {
+        GN_LAUNCH(grid, dim3(GN_THREADS), gn_apply_kernel, true);
+    } else {
+        hipLaunchKernelGGL(gn_join_kernel<false>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
+        GN_LAUNCH(grid, dim3(GN_THREADS), gn_apply_kernel);
+    }
     YOLO_CHECK_HIP(hipGetLastError());
     return YOLO_OK;
 }
@@ -1492,7 +1621,9 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
     p.stream = gn_stream_rule(p, es, 3);
     hipStream_t st = (hipStream_t)stream;
     GnWhole w;
-    if (gn_whole_plan(p, es, true, &w)) {
+    GnParams q = p;
+    const bool joined = gn_split_joined(q, es, true);
+    if (gn_whole_plan(p, es, true, &w) && (!joined || gn_whole_first(p, es, true, w))) {
         p.VS = w.VS;
         p.PL = 64 / w.VS;
         p.slabs = (p.C * es / 16 + w.VS - 1) / w.VS;
@@ -1510,11 +1641,15 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
         YOLO_CHECK_HIP(hipGetLastError());
         return YOLO_OK;
     }
+    if (joined) p = q;
     dim3 grid = gn_grid(p, es);
     GN_LAUNCH(grid, dim3(GN_THREADS), gn_bwd_sums_kernel);
-    hipLaunchKernelGGL(gn_join_kernel<true>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
+    if (!joined) hipLaunchKernelGGL(gn_join_kernel<true>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
     ++grid.z;  // dgamma and dbeta
-    GN_LAUNCH(grid, dim3(GN_THREADS), gn_bwd_apply_kernel);
+    if (joined)
+        GN_LAUNCH(grid, dim3(GN_THREADS), gn_bwd_apply_kernel, true);
+    else
+        GN_LAUNCH(grid, dim3(GN_THREADS), gn_bwd_apply_kernel);
     YOLO_CHECK_HIP(hipGetLastError());
     return YOLO_OK;
 }
