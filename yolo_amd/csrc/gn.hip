@@ -349,6 +349,25 @@ __global__ void __launch_bounds__(GN_THREADS, 5) gn_sums_kernel(const GnParams p
     }
 }
 
+// sum[k] += value k of the rows from, from + step, ... below count, U rows' loads at a time, the last ones too: each row is a trip to
+// memory of 1 us.  load(row, k) is called with rows below count only.
+template <int U, int K, typename P, typename L>
+__device__ __forceinline__ void gn_sum_rows(int from, int count, int step, double (&sum)[K], L load) {
+    for (int i = from; i < count; i += U * step) {
+        P v[U][K];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                v[u][k] = 0;
+                if (i + u * step < count) v[u][k] = load(i + u * step, k);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < K; ++k) sum[k] += (double)v[u][k];
+    }
+}
 __device__ __forceinline__ float gn_rstd(const GnParams& p, double var) {
     return (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps));
 }
@@ -367,13 +386,9 @@ __global__ void __launch_bounds__(GN_JOIN * 64) gn_join_kernel(const GnParams p)
     double A = 0.0, B = 0.0;
     for (int c0 = 0; c0 < width; c0 += 64) {
         const int c = c0 + col;
-        double a = 0.0, b = 0.0;
-        if (c < width)
-#pragma unroll 4
-            for (int i = row; i < p.chunks; i += GN_JOIN) {
-                a += (double)part[(long long)i * 2 * p.C + c];
-                b += (double)part[((long long)i * 2 + 1) * p.C + c];
-            }
+        double sum[2] = {0.0, 0.0};
+        if (c < width) gn_sum_rows<8, 2, P>(row, p.chunks, GN_JOIN, sum, [&](int i, int k) { return part[((long long)i * 2 + k) * p.C + c]; });
+        double a = sum[0], b = sum[1];
         red[0][row][col] = a;
         red[1][row][col] = b;
         __syncthreads();
@@ -415,30 +430,50 @@ __global__ void __launch_bounds__(GN_JOIN * 64) gn_join_kernel(const GnParams p)
 }
 
 // The same for the `width` channels of a slab (whole groups) from c0 on, by a workgroup that goes on with them: the group sums of its
-// groups, handed to done(group in the slab, sum, sum, lane) in 16 lanes each.
+// groups, handed to done(group in the slab, sum, sum, lane) in 16 lanes each.  16 bytes of sums a lane; `red` has room for a workgroup's.
 template <bool BWD, typename F>
-__device__ __forceinline__ void gn_join_slab(const GnParams& p, int n, int c0, int width, double (*red)[GN_THREADS], F done) {
+__device__ __forceinline__ void gn_join_slab(const GnParams& p, int n, int c0, int width, double* red, F done) {
     typedef typename std::conditional<BWD, float, double>::type P;
-    const int rows = GN_THREADS / width, row = threadIdx.x / width, col = threadIdx.x - row * width;
+    constexpr int K = 16 / (int)sizeof(P);  // channels of a lane; width and c0 are multiples of it
+    typedef P PK __attribute__((ext_vector_type(K)));
+    const int lanes = width / K, rows = min(GN_THREADS / lanes, p.chunks), row = threadIdx.x / lanes, col = (threadIdx.x - row * lanes) * K;
     const P* part = (const P*)p.partial + (long long)n * p.chunks * 2 * p.C + c0 + col;
-    double a = 0.0, b = 0.0;
+    double sum[2][K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) sum[0][k] = sum[1][k] = 0.0;
+    constexpr int U = 4;  // rows' loads at a time, the last ones too: each is a trip to memory
     if (row < rows)
-#pragma unroll 8
-        for (int i = row; i < p.chunks; i += rows) {
-            a += (double)part[(long long)i * 2 * p.C];
-            b += (double)part[((long long)i * 2 + 1) * p.C];
+        for (int i = row; i < p.chunks; i += U * rows) {
+            PK v[U][2];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    v[u][w] = PK(0);
+                    if (i + u * rows < p.chunks) v[u][w] = *(const PK*)(part + ((long long)(i + u * rows) * 2 + w) * p.C);
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int k = 0; k < K; ++k) sum[w][k] += (double)v[u][w][k];
         }
-    red[0][threadIdx.x] = a;
-    red[1][threadIdx.x] = b;
-    __syncthreads();
+    double total[2] = {0.0, 0.0};
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        if (row < rows)
+#pragma unroll
+            for (int k = 0; k < K; ++k) red[row * width + col + k] = sum[w][k];
+        __syncthreads();
+        if ((int)threadIdx.x < width)
+            for (int r = 0; r < rows; ++r) total[w] += red[r * width + threadIdx.x];
+        __syncthreads();
+    }
     if ((int)threadIdx.x < width) {
-        for (int r = 1; r < rows; ++r) {
-            a += red[0][r * width + threadIdx.x];
-            b += red[1][r * width + threadIdx.x];
-        }
         const double gamma = BWD ? p.gamma[c0 + threadIdx.x] : 1.f;
-        red[0][threadIdx.x] = gamma * a;
-        red[1][threadIdx.x] = gamma * b;
+        red[threadIdx.x] = gamma * total[0];
+        red[GN_THREADS + threadIdx.x] = gamma * total[1];
     }
     __syncthreads();
     const int sub = threadIdx.x & 15, groups = width / p.Cg;
@@ -447,8 +482,8 @@ __device__ __forceinline__ void gn_join_slab(const GnParams& p, int n, int c0, i
         double A = 0.0, B = 0.0;
         if (g < groups)
             for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) {
-                A += red[0][i];
-                B += red[1][i];
+                A += red[i];
+                B += red[GN_THREADS + i];
             }
         for (int o = 8; o; o >>= 1) {
             A += __shfl_xor(A, o);
@@ -464,7 +499,7 @@ __device__ __forceinline__ void gn_join_slab(const GnParams& p, int n, int c0, i
 template <typename E, int ACT, bool JOIN = false>
 __global__ void __launch_bounds__(GN_THREADS, JOIN ? 6 : 8) gn_apply_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
-    __shared__ double red[2][JOIN ? GN_THREADS : 1];
+    __shared__ double red[JOIN ? 2 * GN_THREADS : 1];
     __shared__ float of[2][JOIN ? GN_THREADS : 1];
     // fp32: (x - mean) * scale + beta; bf16: x * scale + (beta - mean * scale), whose rounding of mean * scale is far below the
     // output's
@@ -474,7 +509,7 @@ __global__ void __launch_bounds__(GN_THREADS, JOIN ? 6 : 8) gn_apply_kernel(cons
     const int n = p.N - 1 - blockIdx.z, chunk = p.chunks - 1 - blockIdx.x;
     const int first = chunk * p.chunk, last = min(first + p.chunk, p.HW), c0 = blockIdx.y * p.VS * V;
     if constexpr (JOIN)
-        gn_join_slab<false>(p, n, c0, min(p.VS * V, p.C - c0), (double (*)[GN_THREADS])red, [&](int g, double A, double B, int sub) {
+        gn_join_slab<false>(p, n, c0, min(p.VS * V, p.C - c0), red, [&](int g, double A, double B, int sub) {
             const double m = A * p.inv_count;
             const float mean = (float)m, r = gn_rstd(p, B * p.inv_count - m * m);
             for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) {
@@ -596,10 +631,9 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_sums_kernel(const GnPara
 // and eight rows at a time.
 __device__ __forceinline__ void gn_params(const GnParams& p, int set, double (*red)[32], const float* sums, int rows) {
     const int col = threadIdx.x & 31, row = threadIdx.x >> 5, i = set * 32 + col;
-    double a = 0.0;
-    if (i < 2 * p.C)
-#pragma unroll 8
-        for (int n = row; n < rows; n += 8) a += (double)sums[(long long)n * 2 * p.C + i];
+    double sum[1] = {0.0};
+    if (i < 2 * p.C) gn_sum_rows<8, 1, float>(row, rows, 8, sum, [&](int n, int) { return sums[(long long)n * 2 * p.C + i]; });
+    double a = sum[0];
     red[row][col] = a;
     __syncthreads();
     if (row == 0 && i < 2 * p.C) {
@@ -636,7 +670,7 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_apply_kernel(const GnPar
     gn_stage(lds, p, n, blockIdx.y * S, S);
     float* terms = lds + 4 * GN_THREADS;  // JOIN: behind the constants of at most GN_THREADS channels; then the sums to join
     if constexpr (JOIN)
-        gn_join_slab<true>(p, n, blockIdx.y * S, min(S, p.C - (int)blockIdx.y * S), (double (*)[GN_THREADS])(lds + 6 * GN_THREADS),
+        gn_join_slab<true>(p, n, blockIdx.y * S, min(S, p.C - (int)blockIdx.y * S), (double*)(lds + 6 * GN_THREADS),
                            [&](int g, double A, double B, int sub) {
                                for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) {
                                    terms[i] = (float)(A * p.inv_count);
