@@ -1459,15 +1459,21 @@ static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out
 
 // Where both are possible, the chunked passes without the joining launch have every CU at work on few images, and whole slabs x in
 // registers.  Measured (us, whole and chunked):
-//   forward   with a residual, 80 KB and more to each of less than 256 workgroups: bf16 1 x 52 x 52 x 256 17.2 and 13.2, 8 images 19.1
-//             and 18.4, 16 (256 workgroups) 26.1 and 27.7, 1 x 26 x 26 x 512 (28 KB) 7.3 and 10.9;  8 without a residual 15.0 and 17.5
-//   backward  bf16, less than 512 slabs of 128 B: 1 x 40 x 40 x 256 20.6 and 11.1, 24 x 13 x 13 x 1024 (384) 18.1 and 16.8, 32 (512) 19.5
-//             and 19.9;  16 MB and less: 16 x 26 x 26 x 512 20.0 and 18.3, 32 (22 MB) 27.2 and 29.2
-//             f32, less than 128: 4 x 26 x 26 x 512 (64) 13.2 and 12.9, 8 x 13 x 13 x 1024 (256) 11.8 and 13.1
+//   forward, with a residual: 48 KB and more to each of less than 256 workgroups: 1 x 52 x 52 x 256 16.9 and 11.9, 8 images 19.1 and
+//             17.4, 16 (256 workgroups) 25.7 and 26.6;  4 x 60 x 60 x 128 20.0 and 12.5;  1 x 40 x 40 x 256 (56 KB) 12.5 and 11.2, 1 x 26 x
+//             26 x 512 (28 KB) 7.3 and 10.8
+//   without one: 80 KB, less than 32: 1 x 52 x 52 x 256 12.2 and 11.6, 8 images 15.0 and 16.6;  1 x 40 x 40 x 256 8.2 and 9.8
+//             112 KB, less than 128: 8 x 64 x 64 x 64 (64) 16.9 and 12.8;  16 x 60 x 60 x 128 (128) 18.1 and 18.4
+//   backward  bf16, less than 512 slabs of 128 B: 1 x 40 x 40 x 256 20.8 and 11.0, 24 x 13 x 13 x 1024 (384) 17.8 and 17.0, 32 (512) 18.9
+//             and 19.9;  16 MB and less: 16 x 26 x 26 x 512 20.0 and 18.6, 32 (22 MB) 26.6 and 29.9
+//             f32, less than 128: 4 x 26 x 26 x 512 (64) 13.4 and 13.2, 8 x 13 x 13 x 1024 (256) 11.8 and 13.1
 static bool gn_whole_first(const GnParams& p, int es, bool backward, const GnWhole& w) {
     const int vecs = p.C * es / 16;
     if (w.tall) return true;
-    if (!backward) return !p.r.p || w.waves * w.NV < 80 || (long long)p.N * ((vecs + w.VS - 1) / w.VS) >= 256;
+    if (!backward) {
+        const int kb = w.waves * w.NV, few = p.r.p ? (kb >= 48 ? 256 : 0) : (kb >= 112 ? 128 : kb >= 80 ? 32 : 0);
+        return (long long)p.N * ((vecs + w.VS - 1) / w.VS) >= few;
+    }
     return (long long)p.N * ((vecs + 7) / 8) >= (es == 2 ? 512 : 128) || (long long)p.N * p.HW * p.C * es > (16ll << 20);
 }
 
