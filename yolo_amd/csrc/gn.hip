@@ -10,9 +10,10 @@
 //             dx = r * (gamma * d - A - xh * B),  A = sum over the group of gamma * d / M,  B = the same of d * xh
 //
 // Memory-bound: some twenty operations for each value of 2 or 4 bytes.  A pass reads or writes 16 bytes per lane, sums are fp32
-// within a thread (about a pivot where squares would cancel) and fp64 from there on.  Two forms, chosen by gn_whole_plan:
+// within a thread (about a pivot where squares would cancel) and fp64 from there on.  Two forms, chosen by gn_whole_plan and gn_whole_first:
 //   whole    a workgroup holds a slab (whole groups) of one image in registers: x and dy are read once, one launch
-//   chunked  an image's slab over many workgroups, with a second pass over x and dy: sums, join, output
+//   chunked  an image's slab over many workgroups, with a second pass over x and dy: sums, join, output (with few chunks the second
+//            pass joins the sums itself: gn_split_joined)
 // No atomics and a fixed order of additions: a call gives the same bits each time.
 #include <type_traits>
 
