@@ -169,7 +169,8 @@ __device__ __forceinline__ float gn_act_grad(float dy, float t, float slope, flo
 // loaded ahead would take.
 __device__ __forceinline__ float gn_exact_side(float x, const float* lds, int c, int row, float slope) {
     asm volatile("" : "+v"(c));
-    float side = ((double)x - (double)lds[c]) * (double)lds[c + row] * (double)lds[c + 2 * row] + (double)lds[c + 3 * row] > 0.0 ? 1.f : slope;
+    const double t = ((double)x - (double)lds[c]) * (double)lds[c + row] * (double)lds[c + 2 * row] + (double)lds[c + 3 * row];
+    float side = t > 0.0 ? 1.f : slope;
     asm volatile("" : "+v"(side));
     return side;
 }
@@ -215,8 +216,8 @@ struct GnConst {
 
 // x - mean and d = dy * act'(t) of a vector's channels; k holds the constants of K of them, the ones from `part` * K on.
 template <typename E, int ACT, int K>
-__device__ __forceinline__ void gn_grads_of(const u32x4& x, const u32x4& dy, int part, const GnConst<K>& k, float near, const float* lds, int c,
-                                            int row, float slope, float* xm, float* a) {
+__device__ __forceinline__ void gn_grads_of(const u32x4& x, const u32x4& dy, int part, const GnConst<K>& k, float near,
+                                            const float* lds, int c, int row, float slope, float* xm, float* a) {
     float least = INFINITY;
     gn_part<E, K>(x, part, xm);
     gn_part<E, K>(dy, part, a);
@@ -388,7 +389,8 @@ __global__ void __launch_bounds__(GN_JOIN * 64) gn_join_kernel(const GnParams p)
     for (int c0 = 0; c0 < width; c0 += 64) {
         const int c = c0 + col;
         double sum[2] = {0.0, 0.0};
-        if (c < width) gn_sum_rows<8, 2, P>(row, p.chunks, GN_JOIN, sum, [&](int i, int k) { return part[((long long)i * 2 + k) * p.C + c]; });
+        if (c < width)
+            gn_sum_rows<8, 2, P>(row, p.chunks, GN_JOIN, sum, [&](int i, int k) { return part[((long long)i * 2 + k) * p.C + c]; });
         double a = sum[0], b = sum[1];
         red[0][row][col] = a;
         red[1][row][col] = b;
@@ -571,7 +573,8 @@ __global__ void __launch_bounds__(GN_THREADS, JOIN ? 6 : 8) gn_apply_kernel(cons
 }
 
 // ------------------------------------------------------------------------------------------------ backward, sums
-// partial[n][chunk][0 / 1][c] = sum of d, of d * xh over the chunk's pixels, two pairs of vectors ahead.  64 x 208 x 208 x 64 bf16: 709 MB in 118 us, 6.0 TB/s.
+// partial[n][chunk][0 / 1][c] = sum of d, of d * xh over the chunk's pixels, two pairs of vectors ahead.  64 x 208 x 208 x
+// 64 bf16: 709 MB in 118 us, 6.0 TB/s.
 template <typename E, int ACT>
 __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_sums_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
