@@ -9,8 +9,9 @@
 //             dbeta = sum over images and pixels of d,  dgamma = the same of d * xh
 //             dx = r * (gamma * d - A - xh * B),  A = sum over the group of gamma * d / M,  B = the same of d * xh
 //
-// Memory-bound: some twenty operations for each value of 2 or 4 bytes.  A pass reads or writes 16 bytes per lane, sums are fp32
-// within a thread (about a pivot where squares would cancel) and fp64 from there on.  Two forms, chosen by gn_whole_plan and gn_whole_first:
+// Memory-bound: some twenty operations for each value of 2 or 4 bytes.  A pass reads or writes 16 bytes per lane.  Forward, sums are
+// of differences from a pivot, fp32 over a thread's values (and a wave's, where a slab is in registers), fp64 from there on; backward
+// they are fp32 within a workgroup.  Two forms, chosen by gn_whole_plan and gn_whole_first:
 //   whole    a workgroup holds a slab (whole groups) of one image in registers: x and dy are read once, one launch
 //   chunked  an image's slab over many workgroups, with a second pass over x and dy: sums, join, output (with few chunks the second
 //            pass joins the sums itself: gn_split_joined)
@@ -726,9 +727,11 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_apply_kernel(const GnPar
 // ------------------------------------------------------------------------------------------------ whole images
 // One workgroup holds all pixels of a slab of whole groups of one image in registers, so that x (and dy) are read once: VS
 // vectors of 16 bytes per pixel, 64 / VS pixels next to each other in a wave, NV vectors to a thread.  The statistics are then
-// the two sums of the definition (mean, then squares about it), fp32 in a thread and fp64 between threads.  64 x 52 x 52 x 256 bf16
-// with a residual: 266 MB in 57 us, 4.7 TB/s (one round of 256 workgroups that load, add up and store at the same time); one image
-// of 13 x 13 x 1024: 6.4 us, of which a launch and the way to memory and back are most.
+// the two sums of the definition (mean, then squares about it), fp32 in a thread, over its channels of a group and over its wave's pixel
+// lanes (at most 22 + 3 + 6 additions in a row), fp64 between waves.  The first sum is of differences from the channel's value at pixel 0:
+// raw values far from zero would lose the mean's last digits, and a nearly constant group (r up to 1 / sqrt(eps)) its output's first
+// ones.  64 x 52 x 52 x 256 bf16 with a residual: 266 MB in 57 us, 4.7 TB/s (one round of 256 workgroups that load, add up and store at
+// the same time); one image of 13 x 13 x 1024: 6.4 us, of which a launch and the way to memory and back are most.
 constexpr int GN_SLAB = 128;  // most channels of a slab (at most the threads of the smallest workgroup)
 constexpr int GN_WAVES = 16;
 
@@ -761,20 +764,17 @@ __device__ __forceinline__ GnSeat gn_seat(const GnParams& p) {
     s.count = s.on && s.first < p.HW ? (p.HW - s.first + s.step - 1) / s.step : 0;
     return s;
 }
-// The thread's vectors of K tensors; where it has none a load repeats its first one (or pixel 0's), so that all of them are plain
-// loads inside the view, issued one after the other.
+// The thread's vectors of K tensors; where it has none a load takes pixel 0's, so that all of them are plain loads inside the view,
+// issued one after the other.
 template <int K>
 struct GnWalk {
     GnCursor<K> c;
-    int at0[K];
+    int at0;
     __device__ __forceinline__ GnWalk(const GnParams& p, const GnSeat& s, int cb, const GnTensor* const (&t)[K])
-        : c(s.count ? s.first : 0, s.step, p.W, cb, t) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) at0[k] = c.at[k];
-    }
+        : c(s.count ? s.first : 0, s.step, p.W, cb, t), at0(cb) {}
     template <int ST, bool ALL>
     __device__ __forceinline__ u32x4 load(int k, int i, const GnSeat& s, const char* base) const {
-        return gn_load<ST>(base, ALL || i < s.count ? c.at[k] : at0[k]);
+        return gn_load<ST>(base, ALL || i < s.count ? c.at[k] : at0);
     }
 };
 // ... and zeros there
@@ -869,6 +869,7 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
     float (*part)[GN_SLAB] = (float (*)[GN_SLAB])parts;
     __shared__ __attribute__((aligned(16))) float mean_of[GN_SLAB], scale_of[GN_SLAB], shift_of[GN_SLAB];  // by channel
     __shared__ double off_of[GN_SLAB];  // by group: the mean minus its fp32 value
+    __shared__ float pivot_of[GN_SLAB];  // by channel: pixel 0's value
     const GnSeat t = gn_seat<E>(p);
     const int n = t.n, S = p.VS * V, c0 = t.slab * S, g0 = c0 / p.Cg, top = gn_top(p.PL), width = min(S, p.C - c0);
     const int groups = width / p.Cg;
@@ -920,7 +921,8 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
             });
         }
     }
-    u32x4 v[NV];
+    // in registers: sums of differences from pixel 0's values (its vector is also what a thread has where it has no pixel)
+    u32x4 v[NV], pivot = gn_load(x, cb);
     gn_with_stream(p.stream, [&](auto st) {
         GnWalk<1> walk(p, t, cb, {&p.x});
 #pragma unroll
@@ -929,19 +931,26 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
             walk.c.next();
         }
     });
-    if constexpr (!TALL) gn_blank<NV>(v, t);
-    float s[V];
+    float s[V], k0[V];
+    GnVec<E>::unpack(pivot, k0);
 #pragma unroll
-    for (int e = 0; e < V; ++e) s[e] = 0.f;
+    for (int e = 0; e < V; ++e) {
+        s[e] = 0.f;
+        if (t.on && t.first == 0) pivot_of[t.cs + e] = k0[e];
+    }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (TALL || i < t.most) {
             float f[V];
             GnVec<E>::unpack(v[i], f);
 #pragma unroll
-            for (int e = 0; e < V; ++e) s[e] += f[e];
+            for (int e = 0; e < V; ++e) s[e] += f[e] - k0[e];
         }
     gn_group_sums<V>(s, part, p, t, groups, top, [&](int g, double sum, int sub) {
+        double at = 0.0;
+        for (int i = sub; i < p.Cg; i += 16) at += (double)pivot_of[g * p.Cg + i];
+        for (int o = 8; o; o >>= 1) at += __shfl_xor(at, o);
+        sum += at * (TALL ? NV * t.step : p.HW);
         const double mean = (TALL ? sum + others[0][g] : sum) * p.inv_count;
         for (int i = sub; i < p.Cg; i += 16) mean_of[g * p.Cg + i] = (float)mean;
         if (sub == 0) {
