@@ -14,10 +14,11 @@ from .test_gpu_gn import OUT, U, _act, ids
 
 pytestmark = pytest.mark.gpu
 
-# one shape for each form of the forward pass: vectors of 16 bytes that a thread of the whole form holds (4, 11, 16, 22), tall slabs;
-# (N, H, W, bytes of a pixel, groups)
+# one shape for each form of the forward pass: vectors of 16 bytes that a thread of the whole form holds (4, 11, 16, 22), tall slabs,
+# chunked passes of two launches and of three; (N, H, W, bytes of a pixel, groups)
 FORMS = {"whole4": (2, 13, 13, 128, 8), "whole11": (32, 26, 26, 1024, 32), "whole16": (256, 40, 40, 128, 8),
-         "whole22": (256, 46, 45, 128, 8), "tall": (256, 59, 51, 128, 8)}
+         "whole22": (256, 46, 45, 128, 8), "tall": (256, 59, 51, 128, 8), "joined": (1, 52, 52, 512, 32),
+         "chunked": (4, 208, 208, 256, 8), "chunked_split_group": (2, 31, 30, 8224, 8)}
 DTYPES = [torch.float32]
 
 

@@ -42,6 +42,7 @@ struct GnParams {
     float* dgamma;
     float* dbeta;
     void* partial;         // forward: double [N][chunks][2][C]; backward: float [N][chunks][2][C]
+    float* pivots;         // forward: [N][C], the values at pixel 0
     float* sums;           // backward: [N][2][C], one image's sums of d and of d * xh
     float* terms;          // backward: [2][N][groups], A and B
     float eps, slope;
@@ -296,14 +297,17 @@ __device__ __forceinline__ GnLane gn_lane(const GnParams& p) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward, sums
-// partial[n][chunk][0 / 1][c] = sum of x, of x * x over the chunk's pixels.  A thread sums differences from the first value
-// it sees (fp32; the values of a few dozen pixels differ from it by about their spread), and goes over to fp64 after that.
+// partial[n][chunk][0 / 1][c] = sum of x - P, of its square over the chunk's pixels, P the channel's value at pixel 0.  A thread sums
+// differences from the first value it sees (fp32; the values of a few dozen pixels differ from it by about their spread), and goes over
+// to fp64 and to P after that: squares about zero would leave the variance of a group that is constant at 1000 off by 1e-4 of eps
+// even in fp64.
 // Bound by the read: 64 x 208 x 208 x 64 bf16, 354 MB in 65 us, 5.4 TB/s.  256 threads, at most 128 pixels to a thread: 2048
 // workgroups, so that a CU has the loads of several in flight.
 template <typename E>
 __global__ void __launch_bounds__(GN_THREADS, 5) gn_sums_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
     __shared__ double red[GN_THREADS * V];
+    __shared__ u32x4 origin[GN_THREADS];  // pixel 0's vector, which needs no registers here during the loop
     const GnLane l = gn_lane<E>(p);
     const int n = blockIdx.z, first = blockIdx.x * p.chunk, last = min(first + p.chunk, p.HW);
     const char* base = p.x.p + n * p.x.img;
@@ -312,10 +316,12 @@ __global__ void __launch_bounds__(GN_THREADS, 5) gn_sums_kernel(const GnParams p
 #pragma unroll
     for (int e = 0; e < V; ++e) k[e] = s[e] = q[e] = 0.f;
     int count = 0;
+    const u32x4 pixel0 = gn_load(base, l.on ? cb : 0);
     if (l.on && first + l.pl < last) {
         GnCursor<1> c(first + l.pl, p.PL, p.W, cb, {&p.x});
         count = (last - first - l.pl + p.PL - 1) / p.PL;
         GnVec<E>::unpack(gn_load(base, c.at[0]), k);
+        origin[threadIdx.x] = pixel0;
         c.next();
         gn_pipelined<4, 1>(
             count - 1,
@@ -335,11 +341,16 @@ __global__ void __launch_bounds__(GN_THREADS, 5) gn_sums_kernel(const GnParams p
             });
     }
     const int S = p.VS * V;
+    float from[V] = {};
+    if (count) GnVec<E>::unpack(origin[threadIdx.x], from);
+    if (blockIdx.x == 0 && l.on && l.pl == 0)
+#pragma unroll
+        for (int e = 0; e < V; ++e) p.pivots[(long long)n * p.C + l.c + e] = from[e];
     double* out = (double*)p.partial + (((long long)n * p.chunks + blockIdx.x) * 2) * p.C + blockIdx.y * S;
     for (int which = 0; which < 2; ++which) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const double K = k[e], sd = s[e];
+            const double K = (double)k[e] - (double)from[e], sd = s[e];
             red[threadIdx.x * V + e] = which == 0 ? count * K + sd : (double)q[e] + K * (2.0 * sd + count * K);
         }
         __syncthreads();
@@ -371,6 +382,11 @@ __device__ __forceinline__ void gn_sum_rows(int from, int count, int step, doubl
             for (int k = 0; k < K; ++k) sum[k] += (double)v[u][k];
     }
 }
+// The sums of x - P and its square over an image's channel -> about P - by
+__device__ __forceinline__ void gn_move_origin(const GnParams& p, double by, double& sum, double& square) {
+    square += by * (2.0 * sum + p.HW * by);
+    sum += p.HW * by;
+}
 __device__ __forceinline__ float gn_rstd(const GnParams& p, double var) {
     return (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)p.eps));
 }
@@ -401,6 +417,10 @@ __global__ void __launch_bounds__(GN_JOIN * 64) gn_join_kernel(const GnParams p)
                 a += red[0][w][col];
                 b += red[1][w][col];
             }
+            if (!BWD && c < width) {  // about the group's pivot, its first channel's
+                const float* P = p.pivots + (long long)n * p.C + g0 * p.Cg;
+                gn_move_origin(p, (double)P[c] - (double)P[c / p.Cg * p.Cg], a, b);
+            }
             if (BWD && c < width) {
                 p.sums[((long long)n * 2) * p.C + g0 * p.Cg + c] = (float)a;
                 p.sums[((long long)n * 2 + 1) * p.C + g0 * p.Cg + c] = (float)b;
@@ -427,9 +447,9 @@ __global__ void __launch_bounds__(GN_JOIN * 64) gn_join_kernel(const GnParams p)
         p.terms[g] = (float)(A * p.inv_count);
         p.terms[p.N * p.groups + g] = (float)(B * p.inv_count);
     } else {
-        const double mean = A * p.inv_count, var = B * p.inv_count - mean * mean;
-        p.stats[g] = (float)mean;
-        p.stats[p.N * p.groups + g] = gn_rstd(p, var);
+        const double d = A * p.inv_count;
+        p.stats[g] = (float)((double)p.pivots[(long long)n * p.C + (g0 + threadIdx.x) * p.Cg] + d);
+        p.stats[p.N * p.groups + g] = gn_rstd(p, B * p.inv_count - d * d);
     }
 }
 
@@ -442,6 +462,11 @@ __device__ __forceinline__ void gn_join_slab(const GnParams& p, int n, int c0, i
     typedef P PK __attribute__((ext_vector_type(K)));
     const int lanes = width / K, rows = min(GN_THREADS / lanes, p.chunks), row = threadIdx.x / lanes, col = (threadIdx.x - row * lanes) * K;
     const P* part = (const P*)p.partial + (long long)n * p.chunks * 2 * p.C + c0 + col;
+    double by = 0.0;  // forward: from the channel's pivot to the group's
+    if (!BWD && (int)threadIdx.x < width) {
+        const float* pivot = p.pivots + (long long)n * p.C + c0;
+        by = (double)pivot[threadIdx.x] - (double)pivot[threadIdx.x / p.Cg * p.Cg];
+    }
     double sum[2][K];
 #pragma unroll
     for (int k = 0; k < K; ++k) sum[0][k] = sum[1][k] = 0.0;
@@ -476,6 +501,7 @@ __device__ __forceinline__ void gn_join_slab(const GnParams& p, int n, int c0, i
     }
     if ((int)threadIdx.x < width) {
         const double gamma = BWD ? p.gamma[c0 + threadIdx.x] : 1.f;
+        if constexpr (!BWD) gn_move_origin(p, by, total[0], total[1]);
         red[threadIdx.x] = gamma * total[0];
         red[GN_THREADS + threadIdx.x] = gamma * total[1];
     }
@@ -514,8 +540,8 @@ __global__ void __launch_bounds__(GN_THREADS, JOIN ? 6 : 8) gn_apply_kernel(cons
     const int first = chunk * p.chunk, last = min(first + p.chunk, p.HW), c0 = blockIdx.y * p.VS * V;
     if constexpr (JOIN)
         gn_join_slab<false>(p, n, c0, min(p.VS * V, p.C - c0), red, [&](int g, double A, double B, int sub) {
-            const double m = A * p.inv_count;
-            const float mean = (float)m, r = gn_rstd(p, B * p.inv_count - m * m);
+            const double d = A * p.inv_count;
+            const float mean = (float)((double)p.pivots[(long long)n * p.C + c0 + g * p.Cg] + d), r = gn_rstd(p, B * p.inv_count - d * d);
             for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) {
                 of[0][i] = mean;
                 of[1][i] = r;
@@ -856,7 +882,7 @@ __device__ __forceinline__ int gn_top(int pl) {  // the first distance of a tree
 
 //
 // TALL: slabs that do not fit.  A thread's first NV vectors are in registers, the next GN_KEPT_FWD in LDS, and what is left is read
-// again; those beyond NV are summed first, as in gn_sums_kernel (pivots; fp64 sums of values and squares), the others by the
+// again; those beyond NV are summed first, as in gn_sums_kernel (pivots; fp64 sums of differences and squares), the others by the
 // definition.  64 x 60 x 60 x 256 bf16 with a residual: 75 us, with 64 B whole 100; without one 50 and 63.  Twelve vectors in
 // registers leave room for the residual's (14: 80 us, 16: 82 us; without one 50 and 49).
 constexpr int GN_KEPT_FWD = 8;
@@ -865,7 +891,8 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
     __shared__ double parts[TALL ? GN_WAVES : GN_WAVES / 2][GN_SLAB];
     __shared__ u32x4 kept[TALL ? GN_KEPT_FWD : 1][TALL ? 1024 : 1];
-    __shared__ double others[2][TALL ? GN_SLAB : 1];  // by group: the sums of the values and squares that are not in registers
+    // by group: the sums of x - P and of its square over what is not in registers, P the pivot of the group's first channel
+    __shared__ double others[2][TALL ? GN_SLAB : 1];
     float (*part)[GN_SLAB] = (float (*)[GN_SLAB])parts;
     __shared__ __attribute__((aligned(16))) float mean_of[GN_SLAB], scale_of[GN_SLAB], shift_of[GN_SLAB];  // by channel
     __shared__ double off_of[GN_SLAB];  // by group: the mean minus its fp32 value
@@ -878,6 +905,15 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
     const float gamma = p.gamma[c0 + mine], beta = p.beta[c0 + mine];
     const char* x = p.x.p + n * p.x.img;
     const int more = TALL ? max(t.count - NV, 0) : 0;
+    // sums in registers are of differences from pixel 0's values (its vector is also what a thread has where it has no pixel)
+    const u32x4 pivot = gn_load(x, cb);
+    auto share_pivot = [&] {
+        float k0[V];
+        GnVec<E>::unpack(pivot, k0);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (t.on && t.first == 0) pivot_of[t.cs + e] = k0[e];
+    };
     if constexpr (TALL) {  // sums of differences from the thread's first value, as gn_sums_kernel
         float k[V], s[V], q[V];
 #pragma unroll
@@ -908,12 +944,14 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
                     }
                 });
         }
+        share_pivot();
+        __syncthreads();
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             double m[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const double K = k[e], sd = s[e];
+                const double K = (double)k[e] - (double)pivot_of[(t.cs + e) / p.Cg * p.Cg], sd = s[e];
                 m[e] = which == 0 ? more * K + sd : (double)q[e] + K * (2.0 * sd + more * K);
             }
             gn_group_sums<V>(m, parts, p, t, groups, top, [&](int g, double sum, int sub) {
@@ -921,8 +959,7 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
             });
         }
     }
-    // in registers: sums of differences from pixel 0's values (its vector is also what a thread has where it has no pixel)
-    u32x4 v[NV], pivot = gn_load(x, cb);
+    u32x4 v[NV];
     gn_with_stream(p.stream, [&](auto st) {
         GnWalk<1> walk(p, t, cb, {&p.x});
 #pragma unroll
@@ -931,13 +968,11 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
             walk.c.next();
         }
     });
+    if constexpr (!TALL) share_pivot();
     float s[V], k0[V];
     GnVec<E>::unpack(pivot, k0);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        s[e] = 0.f;
-        if (t.on && t.first == 0) pivot_of[t.cs + e] = k0[e];
-    }
+    for (int e = 0; e < V; ++e) s[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if (TALL || i < t.most) {
@@ -947,11 +982,12 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
             for (int e = 0; e < V; ++e) s[e] += f[e] - k0[e];
         }
     gn_group_sums<V>(s, part, p, t, groups, top, [&](int g, double sum, int sub) {
+        const double P = pivot_of[g * p.Cg];
         double at = 0.0;
-        for (int i = sub; i < p.Cg; i += 16) at += (double)pivot_of[g * p.Cg + i];
+        for (int i = sub; i < p.Cg; i += 16) at += (double)pivot_of[g * p.Cg + i] - P;
         for (int o = 8; o; o >>= 1) at += __shfl_xor(at, o);
         sum += at * (TALL ? NV * t.step : p.HW);
-        const double mean = (TALL ? sum + others[0][g] : sum) * p.inv_count;
+        const double mean = P + (TALL ? sum + others[0][g] : sum) * p.inv_count;
         for (int i = sub; i < p.Cg; i += 16) mean_of[g * p.Cg + i] = (float)mean;
         if (sub == 0) {
             off_of[g] = mean - (double)(float)mean;
@@ -981,7 +1017,7 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
     }
     gn_group_sums<V>(s, part, p, t, groups, top, [&](int g, double sum, int sub) {
         if constexpr (TALL) {
-            const double m = mean_of[g * p.Cg], count = (double)(p.HW - NV * t.step) * p.Cg;
+            const double m = (double)mean_of[g * p.Cg] - (double)pivot_of[g * p.Cg], count = (double)(p.HW - NV * t.step) * p.Cg;
             sum += others[1][g] + m * (m * count - 2.0 * others[0][g]);
         }
         const double off = off_of[g], var = sum * p.inv_count - off * off;
@@ -1557,13 +1593,14 @@ extern "C" size_t yolo_gn_workspace_bytes(int N, int H, int W, int C, int groups
     yolo_view v{nullptr, H, W, 0, C, 0};
     const int es = (int)elem_size(dtype);
     gn_shape(p, &v, N, C, groups, es);
-    // forward: the double sums; backward: the float sums, then the images' sums and the groups' terms
+    // forward: the double sums, then the pivots; backward: the float sums, then the images' sums and the groups' terms
     auto sums = [&](const GnParams& q, size_t size) { return (size_t)N * q.chunks * 2 * C * size; };
     size_t most = sums(p, sizeof(float)) + ((size_t)N * 2 * C + (size_t)2 * N * groups) * sizeof(float);
     auto more = [&](size_t bytes) { most = bytes > most ? bytes : most; };
-    more(sums(p, sizeof(double)));
+    const size_t pivots = (size_t)N * C * sizeof(float);
+    more(sums(p, sizeof(double)) + pivots);
     GnParams q = p;
-    if (gn_split_joined(q, es, false)) more(sums(q, sizeof(double)));
+    if (gn_split_joined(q, es, false)) more(sums(q, sizeof(double)) + pivots);
     if (gn_split_joined(q, es, true)) more(sums(q, sizeof(float)));
     return most;
 }
@@ -1624,6 +1661,7 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
         return YOLO_OK;
     }
     if (joined) p = q;
+    p.pivots = (float*)((double*)workspace + (size_t)N * p.chunks * 2 * C);
     const dim3 grid = gn_grid(p, es);
     if (dtype == YOLO_BF16)
         hipLaunchKernelGGL((gn_sums_kernel<unsigned short>), grid, dim3(GN_THREADS), 0, st, p);
