@@ -19,7 +19,7 @@ pytestmark = pytest.mark.gpu
 FORMS = {"whole4": (2, 13, 13, 128, 8), "whole11": (32, 26, 26, 1024, 32), "whole16": (256, 40, 40, 128, 8),
          "whole22": (256, 46, 45, 128, 8), "tall": (256, 59, 51, 128, 8), "joined": (1, 52, 52, 512, 32),
          "chunked": (4, 208, 208, 256, 8), "chunked_split_group": (2, 31, 30, 8224, 8)}
-DTYPES = [torch.float32]
+DTYPES = [torch.float32, torch.bfloat16]
 
 
 def _case(cuda, form, dtype, residual, seed):

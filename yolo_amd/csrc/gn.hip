@@ -525,15 +525,14 @@ __device__ __forceinline__ void gn_join_slab(const GnParams& p, int n, int c0, i
 }
 // ------------------------------------------------------------------------------------------------ forward, output
 // y = act((x - mean) * (gamma r) + beta) [+ residual], images and chunks in the reverse order of the sums: what was read last is
-// still in the cache in front of HBM.  64 x 208 x 208 x 64 bf16: 709 MB in 123 us, 5.8 TB/s.
+// still in the cache in front of HBM.  64 x 208 x 208 x 64 bf16: 709 MB in 123 us, 5.8 TB/s.  (x * (gamma r) + (beta - mean gamma r), an
+// operation less, would round mean gamma r: in a nearly constant group of mean 1000 that is 1e-2, in bf16 too more than the output's
+// own rounding.)
 template <typename E, int ACT, bool JOIN = false>
 __global__ void __launch_bounds__(GN_THREADS, JOIN ? 6 : 8) gn_apply_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
     __shared__ double red[JOIN ? 2 * GN_THREADS : 1];
     __shared__ float of[2][JOIN ? GN_THREADS : 1];
-    // fp32: (x - mean) * scale + beta; bf16: x * scale + (beta - mean * scale), whose rounding of mean * scale is far below the
-    // output's
-    constexpr bool SHIFT = sizeof(E) == 2;
     const GnLane l = gn_lane<E>(p);
     // the pass before this one walked forwards: its last chunks are the ones still in the caches
     const int n = p.N - 1 - blockIdx.z, chunk = p.chunks - 1 - blockIdx.x;
@@ -552,13 +551,13 @@ __global__ void __launch_bounds__(GN_THREADS, JOIN ? 6 : 8) gn_apply_kernel(cons
             }
         });
     if (!l.on || first + l.pl >= last) return;
-    float mean[V], scale[V], shift[V];
+    float mean[V], scale[V], beta[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int g = (l.c + e) / p.Cg;
         mean[e] = JOIN ? of[0][l.c - c0 + e] : p.stats[n * p.groups + g];
         scale[e] = p.gamma[l.c + e] * (JOIN ? of[1][l.c - c0 + e] : p.stats[(p.N + n) * p.groups + g]);
-        shift[e] = SHIFT ? fmaf(-mean[e], scale[e], p.beta[l.c + e]) : p.beta[l.c + e];
+        beta[e] = p.beta[l.c + e];
     }
     const int cb = l.c * (int)sizeof(E);
     const char* x = p.x.p + n * p.x.img;
@@ -570,7 +569,7 @@ __global__ void __launch_bounds__(GN_THREADS, JOIN ? 6 : 8) gn_apply_kernel(cons
             float v[V];
             GnVec<E>::unpack(raw, v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[e] = gn_act<ACT>(fmaf(SHIFT ? v[e] : v[e] - mean[e], scale[e], shift[e]), p.slope);
+            for (int e = 0; e < V; ++e) v[e] = gn_act<ACT>(fmaf(v[e] - mean[e], scale[e], beta[e]), p.slope);
             if (res) {
                 float a[V];
                 GnVec<E>::unpack(*res, a);
@@ -886,15 +885,17 @@ __device__ __forceinline__ int gn_top(int pl) {  // the first distance of a tree
 // definition.  64 x 60 x 60 x 256 bf16 with a residual: 75 us, with 64 B whole 100; without one 50 and 63.  Twelve vectors in
 // registers leave room for the residual's (14: 80 us, 16: 82 us; without one 50 and 49).
 constexpr int GN_KEPT_FWD = 8;
-template <typename E, int ACT, int NV, bool TALL = false>
+enum { GN_WHOLE, GN_TALL, GN_TALL_RESIDUAL };
+template <typename E, int ACT, int NV, int FORM = GN_WHOLE>
 __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
     constexpr int V = GnVec<E>::N;
+    constexpr bool TALL = FORM != GN_WHOLE;
     __shared__ double parts[TALL ? GN_WAVES : GN_WAVES / 2][GN_SLAB];
     __shared__ u32x4 kept[TALL ? GN_KEPT_FWD : 1][TALL ? 1024 : 1];
     // by group: the sums of x - P and of its square over what is not in registers, P the pivot of the group's first channel
     __shared__ double others[2][TALL ? GN_SLAB : 1];
     float (*part)[GN_SLAB] = (float (*)[GN_SLAB])parts;
-    __shared__ __attribute__((aligned(16))) float mean_of[GN_SLAB], scale_of[GN_SLAB], shift_of[GN_SLAB];  // by channel
+    __shared__ __attribute__((aligned(16))) float mean_of[GN_SLAB], scale_of[GN_SLAB], beta_of[GN_SLAB];  // by channel
     __shared__ double off_of[GN_SLAB];  // by group: the mean minus its fp32 value
     __shared__ float pivot_of[GN_SLAB];  // by channel: pixel 0's value
     const GnSeat t = gn_seat<E>(p);
@@ -1025,50 +1026,59 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
         for (int i = g * p.Cg + sub; i < (g + 1) * p.Cg; i += 16) scale_of[i] = r;
         if (sub == 0) p.stats[(p.N + n) * p.groups + g0 + g] = r;
     });
-    // fp32: (x - mean) * scale + beta; bf16: x * scale + (beta - mean * scale), whose rounding of mean * scale is far below the
-    // output's
-    constexpr bool SHIFT = sizeof(E) == 2;
     if ((int)threadIdx.x < width) {
-        const float scale = gamma * scale_of[threadIdx.x];
-        scale_of[threadIdx.x] = scale;
-        shift_of[threadIdx.x] = SHIFT ? fmaf(-mean_of[threadIdx.x], scale, beta) : beta;
+        scale_of[threadIdx.x] *= gamma;
+        beta_of[threadIdx.x] = beta;
     }
     __syncthreads();
     if (!t.count) return;
     gn_forget<NV>(v);
-    const char* res = p.r.p ? p.r.p + n * p.r.img : nullptr;
+    const bool residual = TALL ? FORM == GN_TALL_RESIDUAL : p.r.p != nullptr;
+    const char* res = p.r.p + n * p.r.img;  // read where there is one
     char* y = p.y.p + n * p.y.img;
-    float mean[V], scale[V], shift[V];
+    // Where there are no registers for the constants they come from LDS, for four channels of a vector at a time: 64 x 40 x 40 x 256, 16
+    // vectors, with a residual 39.4 -> 37.8 us; 64 x 60 x 60 x 256, tall, with one 80.8 -> 78.0, without one 51.8 and 54.6.
+    constexpr bool KEEP = NV < 16 && FORM != GN_TALL_RESIDUAL;
+    constexpr int K = KEEP ? V : 4;
+    float mean[K], scale[K], bias[K];
     auto constants = [&](int cs) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            if (!SHIFT) mean[e] = mean_of[cs + e];
+        for (int e = 0; e < K; ++e) {
+            mean[e] = mean_of[cs + e];
             scale[e] = scale_of[cs + e];
-            shift[e] = shift_of[cs + e];
+            bias[e] = beta_of[cs + e];
         }
     };
-    constants(t.cs);
+    if (KEEP) constants(t.cs);
     gn_with_stream(p.stream, [&](auto st) {
         constexpr int ST = decltype(st)::value;
         auto put = [&](const u32x4& raw, const u32x4* r, unsigned to) {
-            if constexpr (NV > 16) {  // no registers to keep them: from LDS for each vector
-                int cs = t.cs;
-                asm volatile("" : "+v"(cs));
-                constants(cs);
-            }
-            float f[V];
-            GnVec<E>::unpack(raw, f);
+            u32x4 out;
 #pragma unroll
-            for (int e = 0; e < V; ++e) f[e] = gn_act<ACT>(fmaf(SHIFT ? f[e] : f[e] - mean[e], scale[e], shift[e]), p.slope);
-            if (r) {
-                float a[V];
-                GnVec<E>::unpack(*r, a);
+            for (int h = 0; h < V / K; ++h) {
+                if constexpr (!KEEP) {
+                    int cs = t.cs + h * K;
+                    asm volatile("" : "+v"(cs));
+                    constants(cs);
+                }
+                float f[K];
+                gn_part<E, K>(raw, h, f);
 #pragma unroll
-                for (int e = 0; e < V; ++e) f[e] += a[e];
+                for (int e = 0; e < K; ++e) f[e] = gn_act<ACT>(fmaf(f[e] - mean[e], scale[e], bias[e]), p.slope);
+                if (r) {
+                    float a[K];
+                    gn_part<E, K>(*r, h, a);
+#pragma unroll
+                    for (int e = 0; e < K; ++e) f[e] += a[e];
+                }
+                if constexpr (KEEP)
+                    out = GnVec<E>::pack(f);
+                else
+                    gn_put_four<E>(out, h, f);
             }
-            gn_store<ST>(y, to, GnVec<E>::pack(f));
+            gn_store<ST>(y, to, out);
         };
-        if (res) {  // the residual of the next vectors is on its way while the last ones are finished
+        if (residual) {  // the residual of the next vectors is on its way while the last ones are finished
             // above 16 vectors more would not stay in registers (64 x 52 x 52 x 256: 57.7 us with 1, 60.4 with 2, 65.7 with 4)
             constexpr int AHEAD = NV > 16 ? 1 : 4;
             GnWalk<1> ahead(p, t, cb, {&p.r});
@@ -1103,7 +1113,7 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
             const int there = min(left, GN_KEPT_FWD);
             GnCursor<1> cy(from, t.step, p.W, cb, {&p.y});
             GnCursor<1> cx(from + there * t.step, t.step, p.W, cb, {&p.x});
-            if (res) {
+            if (residual) {
                 GnCursor<1> cr(from, t.step, p.W, cb, {&p.r});
                 int i = 0;
                 gn_pipelined<2, 1>(
@@ -1646,8 +1656,10 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
         p.slabs = (p.C * es / 16 + w.VS - 1) / w.VS;
         p.stream = p.stream && w.VS % 8 == 0;  // whole cache lines only
         const dim3 grid((unsigned)(p.slabs * N));
-        if (w.tall)
-            GN_LAUNCH(grid, dim3(1024), gn_whole_kernel, 12, true);
+        if (w.tall && residual)
+            GN_LAUNCH(grid, dim3(1024), gn_whole_kernel, 12, GN_TALL_RESIDUAL);
+        else if (w.tall)
+            GN_LAUNCH(grid, dim3(1024), gn_whole_kernel, 12, GN_TALL);
         else
         GN_WHOLE_CASE(gn_whole_kernel, 1)
         GN_WHOLE_CASE(gn_whole_kernel, 2)
