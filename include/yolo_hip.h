@@ -400,6 +400,11 @@ int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const float* gamma,
                     const yolo_view* dx, float* dgamma, float* dbeta, int N, int C, int groups, int act,
                     float leaky_slope, int dtype, void* workspace, size_t ws_bytes, void* stream);
 
+/* Introspection for benchmarks and tests: which kernels a call of these sizes launches, "gn_whole_kernel<dtype,vectors,whole>" (or tall),
+ * "gn_kernel<dtype,joined>" (the chunked passes, two launches; chunked: three), with "bwd_" for the backward pass and ",stream" where
+ * loads and stores go past the caches.  residual, backward: 0 or 1. */
+int yolo_gn_kernel_name(int N, int H, int W, int C, int groups, int dtype, int residual, int backward, char* out, int out_len);
+
 /*
  * Gradient norms and clipping over any number of tensors (detectron2's SOLVER.CLIP_GRADIENTS; torch.nn.utils
  * .clip_grad_norm_ and clip_grad_value_).  A device table of runs says which elements a workgroup owns; the runs of one

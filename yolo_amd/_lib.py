@@ -110,6 +110,7 @@ SIGNATURES = {
     # views as byref() or as a view's bytes
     "yolo_gn_act_fwd": (c_int, [c_void_p] * 6 + [c_int, c_int, c_int, c_float, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
     "yolo_gn_act_bwd": (c_int, [c_void_p] * 8 + [c_int, c_int, c_int, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "yolo_gn_kernel_name": (c_int, [c_int] * 8 + [ctypes.c_char_p, c_int]),
     "yolo_grad_norm_workspace_bytes": (c_size_t, [c_int]),
     "yolo_grad_norm": (c_int, [c_void_p, c_int, c_void_p, c_int, c_float, c_float, c_void_p, c_void_p, c_void_p, c_size_t,
                                c_void_p]),

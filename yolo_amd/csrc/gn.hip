@@ -1536,16 +1536,6 @@ static bool gn_whole_first(const GnParams& p, int es, bool backward, const GnWho
     return (long long)p.N * ((vecs + 7) / 8) >= (es == 2 ? 512 : 128) || (long long)p.N * p.HW * p.C * es > (16ll << 20);
 }
 
-static dim3 gn_join_grid(const GnParams& p) {
-    const int per = p.Cg < 64 ? 64 / p.Cg : 1;
-    return dim3((p.groups + per - 1) / per, p.N);
-}
-
-static dim3 gn_grid(const GnParams& p, int es) {
-    const int vecs = p.C * es / 16;
-    return dim3(p.chunks, (vecs + p.VS - 1) / p.VS, p.N);
-}
-
 // A call that moves more than this leaves little of use in the 256 MB cache in front of HBM; its loads and stores go past the
 // caches, and what the first pass over x has left there stays for the second.  Measured (bf16, us): 64 x 208 x 208 x 64 forward
 // 230 -> 193, backward 347 -> 306; 64 x 52 x 52 x 256 forward 47 -> 36; 64 x 13 x 13 x 1024 backward (66 MB) 23.0 -> 21.8; the
@@ -1554,6 +1544,46 @@ static dim3 gn_grid(const GnParams& p, int es) {
 constexpr long long GN_STREAM_BYTES = 64ll << 20;
 static int gn_stream_rule(const GnParams& p, int es, int tensors) {
     return (long long)tensors * p.N * p.HW * p.C * es >= GN_STREAM_BYTES;
+}
+
+// The channels of a vector that always lie in one group: the largest power of two that divides both.
+static int gn_fold(int Cg, int V) {
+    int f = 1;
+    while (f < V && Cg % (2 * f) == 0) f *= 2;
+    return f;
+}
+
+// The form of a call, with the split that goes with it: p holds the chunked one of three launches.  *held: vectors a thread of the
+// whole form has in registers, the instance to launch.
+enum GnForm { GN_FORM_WHOLE, GN_FORM_TALL, GN_FORM_JOINED, GN_FORM_CHUNKED };
+static GnForm gn_form(GnParams& p, int es, bool backward, GnWhole* w, int* held) {
+    p.stream = gn_stream_rule(p, es, backward || p.r.p ? 3 : 2);
+    GnParams q = p;
+    const bool joined = gn_split_joined(q, es, backward);
+    if (!gn_whole_plan(p, es, backward, w) || (joined && !gn_whole_first(p, es, backward, *w))) {
+        if (joined) p = q;
+        return joined ? GN_FORM_JOINED : GN_FORM_CHUNKED;
+    }
+    p.VS = w->VS;
+    p.PL = 64 / w->VS;
+    p.fold = gn_fold(p.Cg, 16 / es);
+    p.slabs = (p.C * es / 16 + w->VS - 1) / w->VS;
+    p.stream = p.stream && w->VS % 8 == 0;  // whole cache lines only
+    static const int fwd[] = {1, 2, 4, 6, 8, 11, 16, 22}, bwd[] = {1, 2, 4, 6, 8};
+    const int* k = backward ? bwd : fwd;
+    while (!w->tall && *k < w->NV) ++k;  // gn_whole_plan keeps to the last one
+    *held = !w->tall ? *k : backward ? 8 : 12;
+    return w->tall ? GN_FORM_TALL : GN_FORM_WHOLE;
+}
+
+static dim3 gn_join_grid(const GnParams& p) {
+    const int per = p.Cg < 64 ? 64 / p.Cg : 1;
+    return dim3((p.groups + per - 1) / per, p.N);
+}
+
+static dim3 gn_grid(const GnParams& p, int es) {
+    const int vecs = p.C * es / 16;
+    return dim3(p.chunks, (vecs + p.VS - 1) / p.VS, p.N);
 }
 
 static void gn_shape(GnParams& p, const yolo_view* x, int N, int C, int groups, int es) {
@@ -1586,16 +1616,9 @@ using namespace yolo;
     } while (0)
 
 #define GN_WHOLE_CASE(KERNEL, K)                          \
-    if (w.NV <= K)                                        \
+    if (held == K)                                        \
         GN_LAUNCH(grid, dim3(w.waves * 64), KERNEL, K);   \
     else
-
-// The channels of a vector that always lie in one group: the largest power of two that divides both.
-static int gn_fold(int Cg, int V) {
-    int f = 1;
-    while (f < V && Cg % (2 * f) == 0) f *= 2;
-    return f;
-}
 
 extern "C" size_t yolo_gn_workspace_bytes(int N, int H, int W, int C, int groups, int dtype) {
     if (N <= 0 || H <= 0 || W <= 0 || C <= 0 || C % 8 || groups <= 0 || C % groups || (long long)H * W >= (1ll << 31)) return 0;
@@ -1644,17 +1667,11 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
     p.partial = workspace;
     p.eps = eps;
     p.slope = leaky_slope;
-    p.stream = gn_stream_rule(p, es, residual ? 3 : 2);
     hipStream_t st = (hipStream_t)stream;
     GnWhole w;
-    GnParams q = p;
-    const bool joined = gn_split_joined(q, es, false);
-    if (gn_whole_plan(p, es, false, &w) && (!joined || gn_whole_first(p, es, false, w))) {
-        p.VS = w.VS;
-        p.PL = 64 / w.VS;
-        p.fold = gn_fold(p.Cg, 16 / es);
-        p.slabs = (p.C * es / 16 + w.VS - 1) / w.VS;
-        p.stream = p.stream && w.VS % 8 == 0;  // whole cache lines only
+    int held;
+    const GnForm form = gn_form(p, es, false, &w, &held);
+    if (form == GN_FORM_WHOLE || form == GN_FORM_TALL) {
         const dim3 grid((unsigned)(p.slabs * N));
         if (w.tall && residual)
             GN_LAUNCH(grid, dim3(1024), gn_whole_kernel, 12, GN_TALL_RESIDUAL);
@@ -1672,14 +1689,13 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
         YOLO_CHECK_HIP(hipGetLastError());
         return YOLO_OK;
     }
-    if (joined) p = q;
     p.pivots = (float*)((double*)workspace + (size_t)N * p.chunks * 2 * C);
     const dim3 grid = gn_grid(p, es);
     if (dtype == YOLO_BF16)
         hipLaunchKernelGGL((gn_sums_kernel<unsigned short>), grid, dim3(GN_THREADS), 0, st, p);
     else
         hipLaunchKernelGGL((gn_sums_kernel<float>), grid, dim3(GN_THREADS), 0, st, p);
-    if (joined) {
+    if (form == GN_FORM_JOINED) {
         GN_LAUNCH(grid, dim3(GN_THREADS), gn_apply_kernel, true);
     } else {
         hipLaunchKernelGGL(gn_join_kernel<false>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
@@ -1721,16 +1737,11 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
     p.sums = (float*)workspace + (size_t)N * p.chunks * 2 * C;
     p.terms = p.sums + (size_t)N * 2 * C;
     p.slope = leaky_slope;
-    p.stream = gn_stream_rule(p, es, 3);
     hipStream_t st = (hipStream_t)stream;
     GnWhole w;
-    GnParams q = p;
-    const bool joined = gn_split_joined(q, es, true);
-    if (gn_whole_plan(p, es, true, &w) && (!joined || gn_whole_first(p, es, true, w))) {
-        p.VS = w.VS;
-        p.PL = 64 / w.VS;
-        p.slabs = (p.C * es / 16 + w.VS - 1) / w.VS;
-        p.stream = p.stream && w.VS % 8 == 0;  // whole cache lines only
+    int held;
+    const GnForm form = gn_form(p, es, true, &w, &held);
+    if (form == GN_FORM_WHOLE || form == GN_FORM_TALL) {
         const dim3 grid((unsigned)(p.slabs * N));
         if (w.tall)
             GN_LAUNCH(grid, dim3(1024), gn_whole_bwd_kernel, 8, true);
@@ -1744,7 +1755,7 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
         YOLO_CHECK_HIP(hipGetLastError());
         return YOLO_OK;
     }
-    if (joined) p = q;
+    const bool joined = form == GN_FORM_JOINED;
     dim3 grid = gn_grid(p, es);
     GN_LAUNCH(grid, dim3(GN_THREADS), gn_bwd_sums_kernel);
     if (!joined) hipLaunchKernelGGL(gn_join_kernel<true>, gn_join_grid(p), dim3(GN_JOIN * 64), 0, st, p);
@@ -1754,5 +1765,25 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
     else
         GN_LAUNCH(grid, dim3(GN_THREADS), gn_bwd_apply_kernel);
     YOLO_CHECK_HIP(hipGetLastError());
+    return YOLO_OK;
+}
+
+extern "C" int yolo_gn_kernel_name(int N, int H, int W, int C, int groups, int dtype, int residual, int backward, char* out, int out_len) {
+    YOLO_REQUIRE(out && out_len > 0, "gn_kernel_name: bad argument");
+    if (int e = gn_check_shape(N, C, groups, YOLO_ACT_LEAKY, 0.f, dtype, "gn_kernel_name")) return e;
+    const int es = (int)elem_size(dtype);
+    YOLO_REQUIRE(H > 0 && W > 0 && (long long)H * W < (1ll << 31) / C / es, "gn_kernel_name: %d x %d x %d", H, W, C);
+    GnParams p{};
+    const yolo_view v{nullptr, H, W, 0, C, 0};
+    gn_shape(p, &v, N, C, groups, es);
+    p.r.p = residual && !backward ? out : nullptr;  // whether there is one is all that counts
+    GnWhole w;
+    int held = 0;
+    const GnForm form = gn_form(p, es, backward != 0, &w, &held);
+    static const char* const forms[] = {"whole", "tall", "joined", "chunked"};
+    char many[16] = "";
+    if (held) snprintf(many, sizeof many, ",%d", held);
+    snprintf(out, (size_t)out_len, "gn_%s%skernel<%s%s,%s%s>", held ? "whole_" : "", backward ? "bwd_" : "", dtype == YOLO_BF16 ? "bf16" : "float",
+             many, forms[form], p.stream ? ",stream" : "");
     return YOLO_OK;
 }

@@ -451,6 +451,15 @@ def gn_workspace_bytes(N: int, H: int, W: int, C: int, groups: int, dtype: torch
     return int(lib().yolo_gn_workspace_bytes(N, H, W, C, groups, dtype_code(dtype)))
 
 
+def gn_kernel_name(N: int, H: int, W: int, C: int, groups: int, dtype: torch.dtype, *, residual: bool = False,
+                   backward: bool = False) -> str:
+    """Short name of the kernels gn_act_fwd (or gn_act_bwd) launches for these sizes."""
+    buf = ctypes.create_string_buffer(128)
+    check(lib().yolo_gn_kernel_name(N, H, W, C, groups, dtype_code(dtype), int(residual), int(backward), buf, 128),
+          "yolo_gn_kernel_name")
+    return buf.value.decode()
+
+
 _pack_view = struct.Struct("Piiiii4x").pack   # a YoloView's bytes, at a quarter of the cost of the ctypes structure
 
 
