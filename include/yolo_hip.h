@@ -384,9 +384,10 @@ int yolo_sgd_step(float* param, const float* grad, float* momentum_buf, const in
  *   t = (x - mean) / sqrt(var + eps) * gamma[c] + beta[c],   y = act(t) [+ residual]
  * with mean and (biased) var over the H*W*C/groups values of each image's group.
  *   stats  [2][N][groups] f32: mean and 1 / sqrt(var + eps), which yolo_gn_act_bwd reads
- * y may be x, and may be residual (an output over part of an input is refused); C is a multiple of 8 and of groups; slope in
- * [0, 1]; one image of a view is below 2 GiB; N is at most 65534 and N * groups below 2^30.
- * workspace: yolo_gn_workspace_bytes, enough for either direction, nothing is kept in it between calls.
+ * y may be x, and may be residual (an output over part of an input is refused); stats, the workspace's first
+ * yolo_gn_workspace_bytes and the vectors lie outside the views' buffers and each other; C is a multiple of 8 and of groups;
+ * slope in [0, 1]; one image of a view is below 2 GiB; N is at most 65534 and N * groups below 2^30.
+ * workspace: enough for either direction, nothing is kept in it between calls.
  */
 size_t yolo_gn_workspace_bytes(int N, int H, int W, int C, int groups, int dtype);
 int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const float* beta, const yolo_view* residual,
@@ -395,7 +396,7 @@ int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const float* beta, c
 
 /* Backward of yolo_gn_act_fwd (without the residual, whose gradient is dy itself): from dy, the saved x and stats writes
  * dx, and dgamma, dbeta [C] f32 (overwritten).  The leaky derivative at t == 0 is slope.  dx may be dy, and may be x;
- * dgamma and dbeta need memory of their own. */
+ * dgamma, dbeta and the workspace need memory of their own. */
 int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const float* gamma, const float* beta, const float* stats,
                     const yolo_view* dx, float* dgamma, float* dbeta, int N, int C, int groups, int act,
                     float leaky_slope, int dtype, void* workspace, size_t ws_bytes, void* stream);

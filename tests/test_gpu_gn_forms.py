@@ -233,3 +233,21 @@ def test_captured_forward_and_backward(cuda, shape):
     for i in (1, 0, 0, 1):
         assert all(torch.equal(a, b) for a, b in zip(run(i, graph.replay), want[i])), i
         run(1 - i, both)
+
+
+def test_adjacent_memory_is_taken(cuda):
+    """Everything of a call end to end in one buffer: nothing is shared, nothing is refused, and the bits are the same."""
+    from yolo_amd import ops
+    shape = N, H, W, C, G = 2, 4, 4, 64, 8
+    x, r, dy, gamma, beta = _inputs(cuda, shape, torch.float32, 9)
+    y, stats = _forward(cuda, shape, x, r, gamma, beta)
+    want = _backward(cuda, shape, x, dy, gamma, beta, stats)
+    sizes = [x.numel()] * 5 + [C] * 4 + [2 * N * G, ops.gn_workspace_bytes(*shape, torch.float32) // 4]
+    bx, br, bdy, by, bdx, bg, bb, dg, db, st, ws = torch.zeros(sum(sizes), device=cuda).split(sizes)
+    for b, t in ((bx, x), (br, r), (bdy, dy), (bg, gamma), (bb, beta)):
+        b.copy_(t.flatten())
+    v = lambda b: ops.View(b.view(N, H, W, C), H, W, 0, C)  # noqa: E731
+    ops.gn_act_fwd(v(bx), bg, bb, v(by), st, ws, groups=G, residual=v(br))
+    ops.gn_act_bwd(v(bdy), v(bx), bg, bb, st, v(bdx), dg, db, ws, groups=G)
+    assert torch.equal(by.view_as(y), y) and torch.equal(st.view_as(stats), stats)
+    assert all(torch.equal(a.view_as(b), b) for a, b in zip((bdx, dg, db), want))

@@ -1402,6 +1402,27 @@ static int gn_check_overlap(const yolo_view* out, const yolo_view* in, int N, in
     return YOLO_OK;
 }
 
+// What a call reads and writes beside its views has memory of its own.  (An output view over an input one: gn_check_overlap.)
+struct GnRange {
+    const char* what;
+    const void* p;
+    size_t bytes;
+    bool written, view;
+};
+static GnRange gn_range(const char* what, const yolo_view* v, int N, int es, bool written) {
+    return GnRange{what, v->ptr, (size_t)N * (v->H + 2 * v->halo) * (v->W + 2 * v->halo) * v->ch_total * es, written, true};
+}
+template <int K>
+static int gn_check_memory(const GnRange (&r)[K], const char* op) {
+    for (int i = 0; i < K; ++i)
+        for (int j = 0; j < i; ++j) {
+            const uintptr_t a = (uintptr_t)r[i].p, b = (uintptr_t)r[j].p;
+            if (!a || !b || (r[i].view && r[j].view) || !(r[i].written || r[j].written)) continue;
+            YOLO_REQUIRE(a + r[i].bytes <= b || b + r[j].bytes <= a, "%s: %s and %s share memory", op, r[j].what, r[i].what);
+        }
+    return YOLO_OK;
+}
+
 static GnTensor gn_tensor(const yolo_view* v, int es) {
     const ViewGeom g = geom_of(*v);
     return GnTensor{(char*)v->ptr + (long long)g.origin * es, g.img_stride * es, g.row_stride * es, g.pix_stride * es};
@@ -1653,9 +1674,13 @@ extern "C" int yolo_gn_act_fwd(const yolo_view* x, const float* gamma, const flo
     if (residual)
         if (int e = gn_check_overlap(y, residual, N, C, es, "gn_act_fwd", "residual")) return e;
     YOLO_REQUIRE((uintptr_t)workspace % 16 == 0, "gn_act_fwd: workspace is not 16-byte aligned");
-    if (ws_bytes < yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype))
-        return fail(YOLO_E_WORKSPACE, "gn_act_fwd: workspace of %zu bytes, %zu needed", ws_bytes,
-                    yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype));
+    const size_t need = yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype), vec = (size_t)C * 4;
+    if (ws_bytes < need) return fail(YOLO_E_WORKSPACE, "gn_act_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    const GnRange memory[] = {gn_range("x", x, N, es, false), gn_range("y", y, N, es, true),
+                              residual ? gn_range("residual", residual, N, es, false) : GnRange{},
+                              {"gamma", gamma, vec, false, false}, {"beta", beta, vec, false, false},
+                              {"stats", stats, (size_t)N * groups * 8, true, false}, {"workspace", workspace, need, true, false}};
+    if (int e = gn_check_memory(memory, "gn_act_fwd")) return e;
     GnParams p{};
     gn_shape(p, x, N, C, groups, es);
     p.x = gn_tensor(x, es);
@@ -1720,9 +1745,13 @@ extern "C" int yolo_gn_act_bwd(const yolo_view* dy, const yolo_view* x, const fl
     YOLO_REQUIRE(dgamma != dbeta && dgamma != gamma && dgamma != beta && dbeta != gamma && dbeta != beta,
                  "gn_act_bwd: dgamma and dbeta need memory of their own");
     YOLO_REQUIRE((uintptr_t)workspace % 16 == 0, "gn_act_bwd: workspace is not 16-byte aligned");
-    if (ws_bytes < yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype))
-        return fail(YOLO_E_WORKSPACE, "gn_act_bwd: workspace of %zu bytes, %zu needed", ws_bytes,
-                    yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype));
+    const size_t need = yolo_gn_workspace_bytes(N, x->H, x->W, C, groups, dtype), vec = (size_t)C * 4;
+    if (ws_bytes < need) return fail(YOLO_E_WORKSPACE, "gn_act_bwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    const GnRange memory[] = {gn_range("x", x, N, es, false), gn_range("dy", dy, N, es, false), gn_range("dx", dx, N, es, true),
+                              {"gamma", gamma, vec, false, false}, {"beta", beta, vec, false, false},
+                              {"stats", stats, (size_t)N * groups * 8, false, false}, {"dgamma", dgamma, vec, true, false},
+                              {"dbeta", dbeta, vec, true, false}, {"workspace", workspace, need, true, false}};
+    if (int e = gn_check_memory(memory, "gn_act_bwd")) return e;
     GnParams p{};
     gn_shape(p, x, N, C, groups, es);
     p.x = gn_tensor(x, es);
