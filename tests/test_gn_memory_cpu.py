@@ -1,4 +1,5 @@
-"""GroupNorm calls whose statistics, workspace, vectors and views share memory, in part too, are refused before any launch (no GPU)."""
+"""GroupNorm calls whose statistics, workspace, vectors and views share memory, in part too, are refused before any launch, and so are
+gradient norms whose outputs and workspace do (no GPU)."""
 import ctypes
 
 import pytest
@@ -37,3 +38,13 @@ BWD += [("dgamma", "ws"), ("dbeta", "ws"), ("dgamma", "dbeta"), ("y", "gamma"), 
 def test_shared_memory_is_refused(backward, pair, shift):
     code, message = _call(backward, **{pair[0]: (pair[1], shift)})
     assert code == -1 and ("share memory" in message or "memory of their own" in message), message
+
+
+@pytest.mark.parametrize("each", [False, True], ids=["all", "each"])
+@pytest.mark.parametrize("clip", [False, True], ids=["norm", "clip"])
+@pytest.mark.parametrize("norms,coefs,ws", [(0, 0, 4096), (0, 4096, 0), (4096, 0, 0), (16, 4096, 0), (4096, 48, 0)], ids=str)
+def test_gradient_norms_over_factors_or_workspace_are_refused(norms, coefs, ws, clip, each):
+    L, base = _lib.lib(), 1 << 20
+    call = L.yolo_grad_clip if clip else L.yolo_grad_norm
+    code = call(2 << 20, 8, 3 << 20 if each else None, 5 if each else 0, 2.0, 1.0, base + norms, base + coefs, base + ws, 64, None)
+    assert code == -1 and "share memory" in L.yolo_last_error().decode()

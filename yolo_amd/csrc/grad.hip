@@ -279,6 +279,12 @@ static int grad_norm_launch(const char* op, bool clip, const yolo_grad_block* bl
         return fail(YOLO_E_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", op, ws_bytes, yolo_grad_norm_workspace_bytes(n_blocks));
     double* partial = (double*)workspace;
     const unsigned outs = tensor_first ? (unsigned)n_tensors : 1u;
+    auto apart = [](const void* a, size_t an, const void* b, size_t bn) {
+        return !a || !b || (uintptr_t)a + an <= (uintptr_t)b || (uintptr_t)b + bn <= (uintptr_t)a;
+    };
+    YOLO_REQUIRE(apart(norms, outs * 4ull, coefs, outs * 4ull) && apart(norms, outs * 4ull, partial, n_blocks * 8ull) &&
+                     apart(coefs, outs * 4ull, partial, n_blocks * 8ull),
+                 "%s: norms, factors and workspace share memory", op);
     const dim3 runs((unsigned)n_blocks);
 #define GRAD_NORM(P)                                                                                                             \
     do {                                                                                                                         \
