@@ -978,6 +978,7 @@ class GradTable:
     n_blocks: int
     first: torch.Tensor      # device, [n_tensors + 1] int32: a tensor's first block
     tensors: list
+    counters: list           # one tensor for each version counter among them (a view has its base's)
 
     @property
     def n_tensors(self) -> int:
@@ -1030,7 +1031,8 @@ def grad_table(tensors: Sequence[torch.Tensor]) -> GradTable:
     rows["tensor"] = owner
     rows["dtype"] = codes[owner]
     both = torch.from_numpy(np.concatenate([rows.view(np.uint8), first.view(np.uint8)])).to(tensors[0].device)
-    return GradTable(both[:rows.nbytes], len(rows), both[rows.nbytes:].view(torch.int32), tensors)
+    counters = {id(b): b for b in (t if t._base is None else t._base for t in tensors) if not b.is_inference()}
+    return GradTable(both[:rows.nbytes], len(rows), both[rows.nbytes:].view(torch.int32), tensors, list(counters.values()))
 
 
 def grad_norm_workspace_bytes(table: GradTable) -> int:
@@ -1072,12 +1074,14 @@ def grad_clip(table: GradTable, norms: torch.Tensor, coefs: torch.Tensor, worksp
     """grad_norm, and the table's tensors multiplied by coefs [1], or each by its own of coefs [n_tensors], in place."""
     check(lib().yolo_grad_clip(*_grad_norm_args("grad_clip", table, norms, workspace, norm_type, per_tensor, max_norm, coefs)),
           "yolo_grad_clip")
+    torch.autograd.graph.increment_version(table.counters)   # written outside autograd's sight
 
 
 def grad_clamp(table: GradTable, value: float) -> None:
     """Clamp the table's tensors to [-value, value] in place."""
     _require_cuda(table.blocks, "grad_clamp")
     check(lib().yolo_grad_clamp(_ptr(table.blocks), table.n_blocks, float(value), _stream()), "yolo_grad_clamp")
+    torch.autograd.graph.increment_version(table.counters)
 
 
 @dataclass
