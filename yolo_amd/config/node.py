@@ -79,7 +79,8 @@ class CfgNode(dict):
             return list(new)
         if isinstance(old, float) and isinstance(new, int) and not isinstance(new, bool):
             return float(new)
-        if isinstance(old, float) and new in ("inf", ".inf"):   # no Python literal, and YAML's only in files
+        # the one key with a norm's order: inf has no Python literal, and a YAML one only in files
+        if key.split(".")[-1] == "NORM_TYPE" and isinstance(old, float) and new in ("inf", ".inf"):
             return float("inf")
         raise ValueError(f"Type mismatch ({type(old)} vs. {type(new)}) for config key: {key}")
 
