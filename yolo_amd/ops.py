@@ -1003,7 +1003,7 @@ def grad_table(tensors: Sequence[torch.Tensor]) -> GradTable:
         raise ValueError("grad_table: no tensors")
     dev = tensors[0].get_device()
     _require_cuda(tensors[0], "grad_table")
-    ptrs, counts, codes, sizes = [], [], [], []
+    ptrs, counts, codes, sizes, counters = [], [], [], [], {}
     for t in tensors:
         if t.get_device() != dev:
             _require_cuda(t, "grad_table")
@@ -1014,6 +1014,9 @@ def grad_table(tensors: Sequence[torch.Tensor]) -> GradTable:
         counts.append(n)
         codes.append(dtype_code(t.dtype))
         sizes.append(t.element_size())
+        base = t._base
+        base = t if base is None else base
+        counters[id(base)] = base
     ptrs, counts, codes, sizes = np.array(ptrs, np.uint64), np.array(counts, np.int64), np.array(codes), np.array(sizes, np.int64)
     lo = np.sort(ptrs[counts > 0])
     hi = np.sort((ptrs + (counts * sizes).astype(np.uint64))[counts > 0])
@@ -1031,8 +1034,8 @@ def grad_table(tensors: Sequence[torch.Tensor]) -> GradTable:
     rows["tensor"] = owner
     rows["dtype"] = codes[owner]
     both = torch.from_numpy(np.concatenate([rows.view(np.uint8), first.view(np.uint8)])).to(tensors[0].device)
-    counters = {id(b): b for b in (t if t._base is None else t._base for t in tensors) if not b.is_inference()}
-    return GradTable(both[:rows.nbytes], len(rows), both[rows.nbytes:].view(torch.int32), tensors, list(counters.values()))
+    counters = [t for t in counters.values() if not t.is_inference()]
+    return GradTable(both[:rows.nbytes], len(rows), both[rows.nbytes:].view(torch.int32), tensors, counters)
 
 
 def grad_norm_workspace_bytes(table: GradTable) -> int:
