@@ -91,7 +91,7 @@ __device__ __forceinline__ unsigned int pack_bf16x2(float lo, float hi) {
 }
 
 // LeakyReLU for a negative-side slope in [0, 1]: max(x, slope * x) is bit-identical to
-// x >= 0 ? x : slope * x there (slope 1 = linear), and costs a packed multiply + one max per element
+// x >= 0 ? x : slope * x there (slope 1 = linear), and costs a multiply and a max per element
 // instead of multiply + compare + select.  Raw v_max_f32 skips the compiler's NaN-canonicalising extra max.
 __device__ __forceinline__ float vmax_raw(float a, float b) {
     float r;
@@ -103,8 +103,8 @@ __device__ __forceinline__ f32x4 leaky4(f32x4 v, float slope) {
     return f32x4{vmax_raw(v[0], m[0]), vmax_raw(v[1], m[1]), vmax_raw(v[2], m[2]), vmax_raw(v[3], m[3])};
 }
 
-// Clears `words` 32-bit words with one small launch.  A kernel and not hipMemsetAsync: memset nodes of a captured HIP graph
-// have given wrong results on replays after the first.
+// Clears `words` 32-bit words with one small launch.  A kernel and not hipMemsetAsync, so that no captured graph depends on a memset
+// node.
 static __global__ void __launch_bounds__(64) clear_words_kernel(unsigned* p, int words) {
     for (int i = threadIdx.x; i < words; i += 64) p[i] = 0u;
 }

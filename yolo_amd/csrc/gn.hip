@@ -141,8 +141,8 @@ __device__ __forceinline__ void gn_with_stream(int stream, F f) {
 
 constexpr int GN_LEAKY = YOLO_ACT_LEAKY, GN_SILU = YOLO_ACT_SILU;
 
-// exp through v_exp_f32 and a 1-ulp reciprocal: both are within a few 2^-24 of the value, far inside what the sums around
-// them keep.  t = -inf and +inf give 0 and 1.
+// exp through v_exp_f32: the product with log2(e) is rounded before it, so that the error grows with t, about (|t| + 2) 2^-24 of the
+// value, and 2^-23 more for the reciprocal: |t| below 10 where it counts.  t = -inf and +inf give 0 and 1.
 __device__ __forceinline__ float gn_sigmoid(float t) { return __builtin_amdgcn_rcpf(1.f + __expf(-t)); }
 
 template <int ACT>
