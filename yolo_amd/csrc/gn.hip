@@ -755,8 +755,8 @@ __global__ void __launch_bounds__(GN_THREADS, 4) gn_bwd_apply_kernel(const GnPar
 // the two sums of the definition (mean, then squares about it), fp32 in a thread, over its channels of a group and over its wave's pixel
 // lanes (at most 22 + 3 + 6 additions in a row), fp64 between waves.  The first sum is of differences from the channel's value at pixel 0:
 // raw values far from zero would lose the mean's last digits, and a nearly constant group (r up to 1 / sqrt(eps)) its output's first
-// ones.  64 x 52 x 52 x 256 bf16 with a residual: 266 MB in 57 us, 4.7 TB/s (one round of 256 workgroups that load, add up and store at
-// the same time); one image of 13 x 13 x 1024: 6.4 us, of which a launch and the way to memory and back are most.
+// ones.  64 x 52 x 52 x 256 bf16 with a residual: 266 MB in 58 us, 4.6 TB/s (one round of 256 workgroups that load, add up and store at
+// the same time); one image of 13 x 13 x 1024: 6.8 us, of which a launch and the way to memory and back are most.
 constexpr int GN_SLAB = 128;  // most channels of a slab (at most the threads of the smallest workgroup)
 constexpr int GN_WAVES = 16;
 
@@ -882,8 +882,8 @@ __device__ __forceinline__ int gn_top(int pl) {  // the first distance of a tree
 //
 // TALL: slabs that do not fit.  A thread's first NV vectors are in registers, the next GN_KEPT_FWD in LDS, and what is left is read
 // again; those beyond NV are summed first, as in gn_sums_kernel (pivots; fp64 sums of differences and squares), the others by the
-// definition.  64 x 60 x 60 x 256 bf16 with a residual: 75 us, with 64 B whole 100; without one 50 and 63.  Twelve vectors in
-// registers leave room for the residual's (14: 80 us, 16: 82 us; without one 50 and 49).
+// definition.  64 x 60 x 60 x 256 bf16 with a residual: 78 us, with 64 B whole 98; without one 51 and 67.  Twelve vectors in
+// registers leave room for the residual's (with 14 and 16 that call took 5 and 7 us longer than with 12, the one without as long).
 constexpr int GN_KEPT_FWD = 8;
 enum { GN_WHOLE, GN_TALL, GN_TALL_RESIDUAL };
 template <typename E, int ACT, int NV, int FORM = GN_WHOLE>
@@ -1163,7 +1163,8 @@ __global__ void __launch_bounds__(1024) gn_whole_kernel(const GnParams p) {
 // and dbeta), the group's two terms, dx.  Four channels at a time, so that the constants of a channel stay few.  In this form
 //   t = (x - mean) * (gamma r) + beta,   dx = d * (gamma r) - (x - mean) * (r r B) - r A.
 //
-// 64 x 13 x 13 x 1024 bf16: 66 MB in 18 us, and 3 us for dgamma and dbeta.
+// 64 x 13 x 13 x 1024 bf16: 66 MB in 21 us (one round of 512 workgroups that load, add up and store together), and 4 us for dgamma and
+// dbeta under a profiler; the call takes 22 us.
 //
 // TALL: slabs that do not fit.  A thread's first NV pairs of vectors are in registers, the next GN_KEPT in LDS, and what is left
 // is read again for dx; those beyond NV are summed first, eight channels at a time, as long as the registers are free.  The call on
@@ -1491,17 +1492,16 @@ static bool gn_split_joined(GnParams& p, int es, bool backward) {
 // Whether (and how) workgroups can hold the slabs of an image.  The slab's width, in bytes of a pixel, decides how whole the cache
 // lines are that a workgroup reads, its height in registers what fits; measured (bf16, 32 groups, time of one call in us):
 //   256 B where that leaves 512 workgroups       64 x 13 x 13 x 1024 backward 21.4, with 128 B 22.5
-//   128 B otherwise                              64 x 52 x 52 x 256 forward 36, with 64 B 49, in chunks 55
-//   narrower (to 32 B) for 256 workgroups        16 x 52 x 52 x 256 forward 16.2 with 32 B, 17.5 with 64 B, 24 with 128 B
-//   64 B so that it fits, no less                64 x 104 x 104 x 128 forward 102 with 32 B, in chunks 97; one image 33 and 18
-// Forward a thread takes up to 11 vectors before the workgroup gets more waves (64 x 26 x 26 x 512: 17.8 us with 8 waves of 11, 23.3
+//   128 B otherwise                              64 x 52 x 52 x 256 forward 40, with 64 B 50, in chunks 56
+//   narrower (to 32 B) for 256 workgroups        16 x 52 x 52 x 256 forward 16.1 with 32 B, 17.4 with 64 B, in chunks 22.3
+//   64 B so that it fits, no less                64 x 104 x 104 x 128 forward 107 with 32 B, in chunks 96
+// Forward a thread takes up to 11 vectors before the workgroup gets more waves (64 x 26 x 26 x 512: 18.1 us with 8 waves of 11, 23.3
 // with 16 of 6); backward it has two tensors' vectors, and spills above 8.  Taller slabs are then held in part, at 128 B a pixel,
 // where the CUs, one slab each, are busy:
 //   backward, half of the CUs and more, to 32    64 x 52 x 52 x 256 68.0, in chunks 83;  32 images 44 and 52;  16 images 37 and 32
 //                                                64 x 40 x 40 x 256 41, with 64 B whole 64
 //   all of them, up to 64 vectors                64 x 76 x 76 x 256 backward 150, in chunks 161;  64 x 76 x 76 x 128 (128 slabs) 91 and 87
-//                                                64 x 76 x 76 x 256 forward 82, in chunks 103;  64 x 88 x 88 x 256 122 and 135
-//                                                32 x 60 x 60 x 256 forward (128 slabs) 32, with 64 B whole 31
+//                                                64 x 76 x 76 x 256 forward 83, in chunks 103;  64 x 88 x 88 x 256 126 and 133
 //   several slabs each, the last round not empty 96 x 52 x 52 x 256 backward (384 slabs) 110, in chunks 117;  80 images (320) 104 and 99
 struct GnWhole {
     int VS, waves, NV;
@@ -1538,12 +1538,12 @@ static bool gn_whole_plan(const GnParams& p, int es, bool backward, GnWhole* out
 }
 
 // Where both are possible, the chunked passes without the joining launch have every CU at work on few images, and whole slabs x in
-// registers.  Measured (us, whole and chunked):
-//   forward, with a residual: 48 KB and more to each of less than 256 workgroups: 1 x 52 x 52 x 256 16.9 and 11.9, 8 images 19.1 and
-//             17.4, 16 (256 workgroups) 25.7 and 26.6;  4 x 60 x 60 x 128 20.0 and 12.5;  1 x 40 x 40 x 256 (56 KB) 12.5 and 11.2, 1 x 26 x
-//             26 x 512 (28 KB) 7.3 and 10.8
-//   without one: 80 KB, less than 32: 1 x 52 x 52 x 256 12.2 and 11.6, 8 images 15.0 and 16.6;  1 x 40 x 40 x 256 8.2 and 9.8
-//             112 KB, less than 128: 8 x 64 x 64 x 64 (64) 16.9 and 12.8;  16 x 60 x 60 x 128 (128) 18.1 and 18.4
+// registers.  Measured (us, whole and chunked; forward: replays of a graph over three sets of buffers):
+//   forward, with a residual: 48 KB and more to each of less than 256 workgroups: 1 x 52 x 52 x 256 11.4 and 9.6, 8 images 17.9 and
+//             16.2, 16 (256 workgroups) 19.3 and 25.1;  4 x 60 x 60 x 128 14.7 and 11.8;  1 x 40 x 40 x 256 (56 KB) 9.1 and 9.6, 1 x 26 x
+//             26 x 512 (28 KB) 7.5 and 9.6
+//   without one: 80 KB, less than 32: 1 x 52 x 52 x 256 10.1 and 9.5, 8 images 13.8 and 15.7;  1 x 40 x 40 x 256 8.2 and 9.5
+//             112 KB, less than 128: 8 x 64 x 64 x 64 (64) 15.3 and 11.8;  16 x 60 x 60 x 128 (128) 16.9 and 17.6
 //   backward  bf16, less than 512 slabs of 128 B: 1 x 40 x 40 x 256 20.8 and 11.0, 24 x 13 x 13 x 1024 (384) 17.8 and 17.0, 32 (512) 18.9
 //             and 19.9;  16 MB and less: 16 x 26 x 26 x 512 20.0 and 18.6, 32 (22 MB) 26.6 and 29.9
 //             f32, less than 128: 4 x 26 x 26 x 512 (64) 13.4 and 13.2, 8 x 13 x 13 x 1024 (256) 11.8 and 13.1
@@ -1559,8 +1559,8 @@ static bool gn_whole_first(const GnParams& p, int es, bool backward, const GnWho
 
 // A call that moves more than this leaves little of use in the 256 MB cache in front of HBM; its loads and stores go past the
 // caches, and what the first pass over x has left there stays for the second.  Measured (bf16, us): 64 x 208 x 208 x 64 forward
-// 230 -> 193, backward 347 -> 306; 64 x 52 x 52 x 256 forward 47 -> 36; 64 x 13 x 13 x 1024 backward (66 MB) 23.0 -> 21.8; the
-// one that lost, 16 x 104 x 104 x 128 forward (88 MB): 31.9 -> 33.4.  A network's training step takes the same time with either.
+// 229 -> 192, backward 347 -> 306; 64 x 52 x 52 x 256 forward 53 -> 40; 64 x 13 x 13 x 1024 backward (66 MB) 23.0 -> 21.8; the
+// one that lost, 16 x 104 x 104 x 128 forward (88 MB): 36.1 -> 36.5.  A network's training step takes the same time with either.
 // Only where a workgroup's stores are whole cache lines: narrower slabs share them, and lose a factor of two and more.
 constexpr long long GN_STREAM_BYTES = 64ll << 20;
 static int gn_stream_rule(const GnParams& p, int es, int tensors) {
