@@ -79,8 +79,9 @@ def _grads(parameters) -> List[torch.Tensor]:
 @torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ for gradients on the GPU: scales them in place so that their common norm (1, 2 or inf)
-    is at most ``max_norm`` and returns the norm it was, as a 0-d tensor that nothing has read back.  A training loop that
-    keeps its gradient tensors saves the table with a GradientClipper."""
+    is at most ``max_norm`` and returns the norm it was, as a 0-d tensor that nothing has read back.  Each call builds the
+    table of the gradients and copies it synchronously (the host waits for what is queued before it; not in a captured
+    graph): a training loop that keeps its gradient tensors saves that with a GradientClipper."""
     grads = _grads(parameters)
     if not grads:
         return torch.zeros(())
@@ -103,7 +104,8 @@ class ArenaSGD(torch.optim.SGD):
 
     ``clip`` = (type, value, norm type) clips the gradients in front of the update (GradientClipper's types).  In the
     one-launch step the update reads them through the clip factors and leaves ``.grad`` as backward wrote it; in torch's own
-    step they are clipped in place first, as detectron2 does."""
+    step they are clipped in place first, as detectron2 does, by a clipper built in each step (its table's copy waits for the
+    work queued before it)."""
 
     def __init__(self, params, model=None, clip: Optional[Tuple[str, float, float]] = None, **kw):
         super().__init__(params, **kw)
